@@ -72,6 +72,7 @@ class BoktAttrs(ctypes.Structure):
 
 
 _VP, _I32, _I64, _F32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+_F64 = ctypes.c_double
 _PP = ctypes.POINTER(BoktParams)
 
 SIGNATURES = {
@@ -84,6 +85,15 @@ SIGNATURES = {
     "bokt_rmsnorm_row_scale": (_I32, [_VP, _VP, _I32, _I32, _F32, _I32, _VP]),
     "bokt_gemm_row_scaled": (_I32, [_VP, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _PP, _VP]),
     "bokt_rmsnorm_gemm": (_I32, [_VP, _VP, _VP, _VP, _I32, _I32, _I32, _F32, _I32, _PP, _VP]),
+    "bokt_qk_norm_rope": (
+        _I32, [_VP] * 5 + [_I32, _VP, _I32, _VP, _VP] + [_I32] * 5 + [_VP, _I32, _F32, _I32, _VP]),
+    "bokt_qk_norm_rope_workspace_bytes": (_I64, [_I32]),
+    "bokt_qk_norm_rope_backward": (
+        _I32,
+        [_VP] * 7 + [_I32, _VP, _I32] + [_VP] * 4 + [_I32] * 5
+        + [_VP, _I32, _F32, _I32, _VP, _I64, _VP],
+    ),
+    "bokt_rope_table": (_I32, [_VP, _I32, _I32, _F64, _VP]),
     "bokt_moe_grouped_gemm": (
         _I32,
         [_VP, _VP, _VP, _I32, _VP, _I32, _I32, _I32, _I32, _I32, _I32, _PP, _VP],

@@ -18,6 +18,7 @@
 #include "gemm_tc2.cuh"
 #include "moe_route.cuh"
 #include "norm_gemm.cuh"
+#include "qk_norm_rope.cuh"
 #include "rmsnorm.cuh"
 
 namespace {
@@ -1477,3 +1478,184 @@ extern "C" int bokt_moe_route_noalloc(const int32_t* expert_ids, int A, int E, i
   return launch_route(expert_ids, A, E, scratch, counts, offsets, offsets64, perm, inv_perm, s,
                       "moe_route_noalloc launch");
 }
+
+// ----------------------------------------------------------------- query/key norm + rotation
+namespace {
+
+// Blocks per SM of the persistent backward kernel (its partial rows are sized by this).
+constexpr int kQkGradBlocksPerSm = 4;
+
+bool qk_strides_vec(const bokt::QkSide& s) {
+  return ((s.x_row | s.x_head | s.g_row | s.g_head | s.out_row | s.out_head) & 7) == 0 &&
+         aligned16(s.x) && aligned16(s.g) && aligned16(s.out) && aligned16(s.w);
+}
+
+template <typename T, bool PAIRS, bool GRAD>
+cudaError_t launch_qk_any(const bokt::QkArgs& a, int sm_count, int* blocks, cudaStream_t s) {
+  const long long rows = (long long)a.tokens * max(a.side[0].heads, a.side[1].heads);
+  long long grid = (rows + 3) / 4;
+  if (grid > (long long)kQkGradBlocksPerSm * sm_count) grid = (long long)kQkGradBlocksPerSm * sm_count;
+  *blocks = int(grid);
+  return launch(bokt::qk_norm_rope_any_kernel<T, PAIRS, GRAD>, dim3(unsigned(grid)), dim3(128),
+                size_t(4) * 3 * a.dim * 4, s, a);
+}
+
+template <typename T, int L, bool PAIRS, int R, bool GRAD>
+cudaError_t launch_qk_vec(const bokt::QkArgs& a, int sm_count, int* blocks, cudaStream_t s) {
+  constexpr int hpu = 32 / L * R;
+  const long long u0 = (long long)a.tokens * ((a.side[0].heads + hpu - 1) / hpu);
+  const long long u1 = (long long)a.tokens * ((a.side[1].heads + hpu - 1) / hpu);
+  if constexpr (GRAD) {
+    long long grid = ((u0 > u1 ? u0 : u1) + bokt::kQkWarps - 1) / bokt::kQkWarps;
+    if (grid > (long long)kQkGradBlocksPerSm * sm_count)
+      grid = (long long)kQkGradBlocksPerSm * sm_count;
+    *blocks = int(grid);
+    return launch(bokt::qk_norm_rope_grad_kernel<T, L, PAIRS, R>, dim3(unsigned(grid)),
+                  dim3(bokt::kQkThreads), 0, s, a);
+  } else {
+    *blocks = 0;
+    return launch(bokt::qk_norm_rope_kernel<T, L, PAIRS, R>,
+                  dim3(unsigned((u0 + u1 + bokt::kQkWarps - 1) / bokt::kQkWarps)),
+                  dim3(bokt::kQkThreads), 0, s, a);
+  }
+}
+
+template <typename T, bool PAIRS, bool GRAD>
+cudaError_t launch_qk(const bokt::QkArgs& a, bool vec, int sm_count, int* blocks, cudaStream_t s) {
+  if (!vec) return launch_qk_any<T, PAIRS, GRAD>(a, sm_count, blocks, s);
+  // Few head rows: one row per lane group, so that the call spreads over the
+  // SMs; many: four rows share a token's angles and keep four loads in flight.
+  const bool few = (long long)a.tokens * (a.side[0].heads + a.side[1].heads) < 64ll * sm_count;
+#define BOKT_QK(L) \
+  (few ? launch_qk_vec<T, L, PAIRS, 1, GRAD>(a, sm_count, blocks, s) \
+       : launch_qk_vec<T, L, PAIRS, 4, GRAD>(a, sm_count, blocks, s))
+  if (a.dim <= 64) return BOKT_QK(8);
+  if (a.dim <= 128) return BOKT_QK(16);
+  return BOKT_QK(32);
+#undef BOKT_QK
+}
+
+int qk_norm_rope_impl(bokt::QkArgs* a, const int64_t* strides, int interleaved, int dtype,
+                      bool grad, void* stream, int* blocks, DeviceInfo* dev) {
+  if (dtype != BOKT_FP16 && dtype != BOKT_BF16) return fail(BOKT_ERR_INVALID, "dtype %d", dtype);
+  if (a->tokens < 0 || a->side[0].heads < 0 || a->side[1].heads < 0 || a->table_rows < 0)
+    return fail(BOKT_ERR_INVALID, "negative size");
+  if (a->dim < 2 || a->dim > bokt::kQkMaxDim)
+    return fail(BOKT_ERR_UNSUPPORTED, "head size must be in [2, %d] (got %d)", bokt::kQkMaxDim, a->dim);
+  if (a->rot < 2 || a->rot > a->dim || (a->rot & 1))
+    return fail(BOKT_ERR_INVALID, "rot must be even and in [2, head size] (got %d)", a->rot);
+  if (!(a->eps >= 0.f) || !(a->eps < 3.0e38f))
+    return fail(BOKT_ERR_INVALID, "eps must be finite >= 0");
+  if ((long long)a->tokens * ((long long)a->side[0].heads + a->side[1].heads) > 0x7fffffffLL)
+    return fail(BOKT_ERR_UNSUPPORTED, "more than 2^31 - 1 head rows");
+  *blocks = 0;
+  int rc = device_info(dev);
+  if (rc) return rc;
+  if (a->tokens == 0 || a->side[0].heads + a->side[1].heads == 0) return BOKT_OK;
+  if (!strides || !a->positions || !a->cos_sin) return fail(BOKT_ERR_INVALID, "null pointer");
+  bool vec = a->dim % 8 == 0 && a->dim <= bokt::kQkMaxVecDim && a->rot % (interleaved ? 8 : 16) == 0 &&
+             aligned16(a->cos_sin);
+  for (int i = 0; i < 2; ++i) {
+    bokt::QkSide& s = a->side[i];
+    if (s.heads && (!s.x || !s.w || !s.out || (grad && !s.g)))
+      return fail(BOKT_ERR_INVALID, "null pointer");
+    const int64_t* st = strides + (grad ? 6 : 4) * i;
+    s.x_row = st[0], s.x_head = st[1];
+    s.out_row = st[2], s.out_head = st[3];
+    if (grad) s.g_row = st[4], s.g_head = st[5];
+    vec = vec && (s.heads == 0 || qk_strides_vec(s));
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+#define BOKT_QK(T, P) \
+  (grad ? launch_qk<T, P, true>(*a, vec, dev->sm_count, blocks, s) \
+        : launch_qk<T, P, false>(*a, vec, dev->sm_count, blocks, s))
+  if (dtype == BOKT_BF16)
+    e = interleaved ? BOKT_QK(__nv_bfloat16, true) : BOKT_QK(__nv_bfloat16, false);
+  else
+    e = interleaved ? BOKT_QK(__half, true) : BOKT_QK(__half, false);
+#undef BOKT_QK
+  if (e != cudaSuccess) return cuda_fail(e, "qk_norm_rope launch");
+  return BOKT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bokt_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                      const void* positions, int positions_i64, const float* cos_sin,
+                      int table_rows, void* q_out, void* k_out, int tokens, int heads,
+                      int kv_heads, int dim, int rot, const int64_t* strides, int interleaved,
+                      float eps, int dtype, void* stream) {
+  g_err[0] = 0;
+  bokt::QkArgs a = {};
+  a.side[0].x = q, a.side[0].w = q_weight, a.side[0].out = q_out, a.side[0].heads = heads;
+  a.side[1].x = k, a.side[1].w = k_weight, a.side[1].out = k_out, a.side[1].heads = kv_heads;
+  a.positions = positions, a.positions_i64 = positions_i64;
+  a.cos_sin = cos_sin, a.table_rows = table_rows;
+  a.tokens = tokens, a.dim = dim, a.rot = rot, a.eps = eps;
+  int blocks;
+  DeviceInfo dev;
+  return qk_norm_rope_impl(&a, strides, interleaved, dtype, false, stream, &blocks, &dev);
+}
+
+int64_t bokt_qk_norm_rope_workspace_bytes(int dim) {
+  g_err[0] = 0;
+  DeviceInfo dev;
+  if (device_info(&dev)) return -1;
+  return (int64_t)kQkGradBlocksPerSm * dev.sm_count * 2 * dim * 4;
+}
+
+int bokt_qk_norm_rope_backward(const void* dq_out, const void* dk_out, const void* q,
+                               const void* k, const void* q_weight, const void* k_weight,
+                               const void* positions, int positions_i64, const float* cos_sin,
+                               int table_rows, void* dq, void* dk, float* dq_weight,
+                               float* dk_weight, int tokens, int heads, int kv_heads, int dim,
+                               int rot, const int64_t* strides, int interleaved, float eps,
+                               int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  bokt::QkArgs a = {};
+  a.side[0].x = q, a.side[0].g = dq_out, a.side[0].w = q_weight, a.side[0].out = dq;
+  a.side[1].x = k, a.side[1].g = dk_out, a.side[1].w = k_weight, a.side[1].out = dk;
+  a.side[0].heads = heads, a.side[1].heads = kv_heads;
+  a.positions = positions, a.positions_i64 = positions_i64;
+  a.cos_sin = cos_sin, a.table_rows = table_rows;
+  a.tokens = tokens, a.dim = dim, a.rot = rot, a.eps = eps;
+  a.partials = static_cast<float*>(workspace);
+  if (!dq_weight || !dk_weight || !workspace) return fail(BOKT_ERR_INVALID, "null pointer");
+  DeviceInfo dev;
+  int rc = device_info(&dev);
+  if (rc) return rc;
+  if (workspace_bytes < (int64_t)kQkGradBlocksPerSm * dev.sm_count * 2 * dim * 4)
+    return fail(BOKT_ERR_INVALID, "workspace too small (%lld bytes)", (long long)workspace_bytes);
+  int blocks;
+  rc = qk_norm_rope_impl(&a, strides, interleaved, dtype, true, stream, &blocks, &dev);
+  if (rc) return rc;
+  // No rows: the weight gradients are zero.
+  cudaError_t e = launch(bokt::qk_norm_rope_dweight_kernel, dim3(unsigned((dim + 31) / 32), 2),
+                         dim3(32, 32), 0, static_cast<cudaStream_t>(stream), a.partials, blocks,
+                         dim, dq_weight, dk_weight);
+  if (e != cudaSuccess) return cuda_fail(e, "qk_norm_rope_dweight launch");
+  return BOKT_OK;
+}
+
+int bokt_rope_table(float* cos_sin, int rows, int rot, double base, void* stream) {
+  g_err[0] = 0;
+  if (rows < 0 || rot < 2 || (rot & 1)) return fail(BOKT_ERR_INVALID, "bad size");
+  if (!(base > 0.0) || !(base < 1e300)) return fail(BOKT_ERR_INVALID, "base must be finite > 0");
+  if (rows == 0) return BOKT_OK;
+  if (!cos_sin) return fail(BOKT_ERR_INVALID, "null pointer");
+  DeviceInfo dev;
+  int rc = device_info(&dev);
+  if (rc) return rc;
+  const long long n = (long long)rows * (rot / 2);
+  long long blocks = (n + 255) / 256;
+  if (blocks > 8LL * dev.sm_count) blocks = 8LL * dev.sm_count;
+  cudaError_t e = launch(bokt::rope_table_kernel, dim3(unsigned(blocks)), dim3(256), 0,
+                         static_cast<cudaStream_t>(stream), cos_sin, rows, rot, base);
+  if (e != cudaSuccess) return cuda_fail(e, "rope_table launch");
+  return BOKT_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,401 @@
+// RMSNorm of every query and key head and the rotary position rotation, in one
+// pass, forward and backward (sm_100a).
+//
+// Per token t and head h, with x = q[t, h, :] (or k[t, h, :]), head size D, and
+// c_i, s_i the table's cosine and sine of token t's position:
+//   n = x * rsqrt(mean(x^2) + eps),   y = n * w                        (fp32)
+//   out[a_i] = y[a_i] c_i - y[b_i] s_i,  out[b_i] = y[b_i] c_i + y[a_i] s_i
+// for i < rot / 2, with (a_i, b_i) = (i, i + rot / 2), or (2 i, 2 i + 1) when
+// the pairs are interleaved; out = y past rot.  One rounding, on store.
+// Backward, with g the incoming gradient turned back by the same angle:
+//   dw = sum over tokens and heads of g n          (fp32, fixed order)
+//   dx = r (g w - n mean(g w n)),   r = rsqrt(mean(x^2) + eps)
+// The statistics are recomputed from x, so nothing is saved by the forward pass.
+//
+// HBM bound: x in and out once (backward: x, the gradient, dx).  A head row is
+// D / 8 lanes of one warp, 16 bytes each (L = 8, 16 or 32 lanes, the smallest
+// that holds D), so the row lives in registers, its mean takes log2(L)
+// shuffles, and a rotation partner is another lane's register.  A warp takes
+// 32 / L x R heads of one token: the token's angles are loaded once into 16
+// registers and serve all of them, and R row loads are in flight per lane.
+#pragma once
+
+#include "bokt_device.cuh"
+
+namespace bokt {
+
+constexpr int kStatusBadPosition = 5;
+constexpr int kQkThreads = 256;
+constexpr int kQkWarps = kQkThreads / 32;
+constexpr int kQkMaxVecDim = 256;
+constexpr int kQkMaxDim = 1024;
+
+// One of the two operands (queries or keys); strides in elements.
+struct QkSide {
+  const void* x;
+  const void* g;  // backward: gradient of the output
+  const void* w;  // [D]
+  void* out;      // forward: result, backward: gradient of x
+  int64_t x_row, x_head, g_row, g_head, out_row, out_head;
+  int heads;
+};
+
+struct QkArgs {
+  QkSide side[2];
+  const void* positions;
+  int positions_i64;
+  const float* cos_sin;  // [table_rows][rot]: rot / 2 cosines, then rot / 2 sines
+  int table_rows;
+  int tokens, dim, rot;
+  float eps;
+  float* partials;  // backward: [gridDim.x][2][dim]
+};
+
+__device__ __forceinline__ long long qk_position(const QkArgs& a, int t) {
+  return a.positions_i64 ? reinterpret_cast<const long long*>(a.positions)[t]
+                         : static_cast<long long>(reinterpret_cast<const int32_t*>(a.positions)[t]);
+}
+
+template <typename T>
+__device__ __forceinline__ void qk_unpack(const uint4& v, float (&f)[8]) {
+  float2 p = Pack2<T>::unpack(v.x);
+  f[0] = p.x, f[1] = p.y;
+  p = Pack2<T>::unpack(v.y);
+  f[2] = p.x, f[3] = p.y;
+  p = Pack2<T>::unpack(v.z);
+  f[4] = p.x, f[5] = p.y;
+  p = Pack2<T>::unpack(v.w);
+  f[6] = p.x, f[7] = p.y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 qk_pack(const float (&f)[8]) {
+  return make_uint4(Pack2<T>::pack(f[0], f[1]), Pack2<T>::pack(f[2], f[3]),
+                    Pack2<T>::pack(f[4], f[5]), Pack2<T>::pack(f[6], f[7]));
+}
+
+template <int L>
+__device__ __forceinline__ float qk_row_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The angles of one token as this lane needs them: element j of the lane turns
+// with c[j] and its partner enters with s[j] (the sign of the forward rotation
+// is in s).
+struct QkAngles {
+  float c[8], s[8];
+};
+
+template <bool PAIRS>
+__device__ __forceinline__ void qk_load_angles(const float* row, int rot, int i, QkAngles& a) {
+  if constexpr (PAIRS) {
+    const float4 c = *reinterpret_cast<const float4*>(row + i / 2);
+    const float4 s = *reinterpret_cast<const float4*>(row + rot / 2 + i / 2);
+    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a.c[2 * j] = a.c[2 * j + 1] = cc[j];
+      a.s[2 * j] = -ss[j];
+      a.s[2 * j + 1] = ss[j];
+    }
+  } else {
+    const bool low = i < rot / 2;
+    const int f = low ? i : i - rot / 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 c = *reinterpret_cast<const float4*>(row + f + 4 * h);
+      const float4 s = *reinterpret_cast<const float4*>(row + rot / 2 + f + 4 * h);
+      a.c[4 * h] = c.x, a.c[4 * h + 1] = c.y, a.c[4 * h + 2] = c.z, a.c[4 * h + 3] = c.w;
+      a.s[4 * h] = low ? -s.x : s.x;
+      a.s[4 * h + 1] = low ? -s.y : s.y;
+      a.s[4 * h + 2] = low ? -s.z : s.z;
+      a.s[4 * h + 3] = low ? -s.w : s.w;
+    }
+  }
+}
+
+// v <- v c + partner(v) s (dir = 1) or v c - partner(v) s (dir = -1: the
+// transposed rotation).  Lanes past rot keep v; every lane takes part in the
+// shuffles.  `partner`: the lane that holds the other halves' elements.
+template <bool PAIRS>
+__device__ __forceinline__ void qk_rotate(float (&v)[8], const QkAngles& a, bool turns, int partner,
+                                          float dir) {
+  float o[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    o[j] = PAIRS ? v[j ^ 1] : __shfl_sync(0xffffffffu, v[j], partner);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (turns) v[j] = fmaf(v[j], a.c[j], dir * (o[j] * a.s[j]));
+}
+
+// Head units: unit u covers heads [chunk * HPU, +HPU) of token u / chunks.
+template <typename T, int L, bool PAIRS, int R>
+__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs args) {
+  constexpr int S = 32 / L;
+  pdl_allow_next();
+  const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
+  const int i = l * 8;
+  const float inv_dim = 1.f / args.dim;
+  const bool active = i < args.dim;
+  const bool turns = i < args.rot;
+  const int half = args.rot / 16;
+  const int partner = PAIRS || !turns ? lane : (i < args.rot / 2 ? lane + half : lane - half);
+  const int chunks0 = (args.side[0].heads + S * R - 1) / (S * R);
+  const int chunks1 = (args.side[1].heads + S * R - 1) / (S * R);
+  const int units0 = args.tokens * chunks0;
+  int u = blockIdx.x * kQkWarps + (threadIdx.x >> 5);
+  if (u >= units0 + args.tokens * chunks1) return;
+  const QkSide& sd = args.side[u >= units0];
+  const int chunks = u >= units0 ? chunks1 : chunks0;
+  if (u >= units0) u -= units0;
+  const int t = u / chunks;
+  const int h0 = (u - t * chunks) * S * R + sub;
+  pdl_wait();
+  const T* x = static_cast<const T*>(sd.x) + t * sd.x_row + i;
+  uint4 raw[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int h = h0 + r * S;
+    raw[r] = active && h < sd.heads ? *reinterpret_cast<const uint4*>(x + h * sd.x_head)
+                                    : make_uint4(0, 0, 0, 0);
+  }
+  const long long pos = qk_position(args, t);
+  float w[8];
+  qk_unpack<T>(active ? *reinterpret_cast<const uint4*>(static_cast<const T*>(sd.w) + i)
+                      : make_uint4(0, 0, 0, 0), w);
+  if (pos < 0 || pos >= args.table_rows) {
+    if (lane == 0) report_status(kStatusBadPosition, t);
+    return;
+  }
+  QkAngles ang = {};
+  if (turns) qk_load_angles<PAIRS>(args.cos_sin + pos * args.rot, args.rot, i, ang);
+  T* out = static_cast<T*>(sd.out) + t * sd.out_row + i;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int h = h0 + r * S;
+    float v[8], ss = 0.f;
+    qk_unpack<T>(raw[r], v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+    const float rs = rsqrtf(fmaf(qk_row_sum<L>(ss), inv_dim, args.eps));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * rs * w[j];
+    qk_rotate<PAIRS>(v, ang, turns, partner, 1.f);
+    if (active && h < sd.heads) *reinterpret_cast<uint4*>(out + h * sd.out_head) = qk_pack<T>(v);
+  }
+}
+
+// Backward: persistent warps walk the query units, then the key units; the
+// weight gradient of a side stays in 8 registers per lane until its last unit,
+// is summed over the block's rows in shared memory and leaves as one partial
+// row per block, which qk_norm_rope_dweight_kernel adds in block order.
+template <typename T, int L, bool PAIRS, int R>
+__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_grad_kernel(const QkArgs args) {
+  constexpr int S = 32 / L;
+  __shared__ float sums[kQkWarps * S][L * 8 + 1];
+  pdl_allow_next();
+  const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L, warp = threadIdx.x >> 5;
+  const int i = l * 8;
+  const float inv_dim = 1.f / args.dim;
+  const bool active = i < args.dim;
+  const bool turns = i < args.rot;
+  const int half = args.rot / 16;
+  const int partner = PAIRS || !turns ? lane : (i < args.rot / 2 ? lane + half : lane - half);
+  pdl_wait();
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    const QkSide& sd = args.side[side];
+    const int chunks = (sd.heads + S * R - 1) / (S * R);
+    const int units = args.tokens * chunks;
+    float w[8], dw[8] = {};
+    qk_unpack<T>(active && units > 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(sd.w) + i)
+                                     : make_uint4(0, 0, 0, 0), w);
+#pragma unroll 1
+    for (int u = blockIdx.x * kQkWarps + warp; u < units; u += gridDim.x * kQkWarps) {
+      const int t = u / chunks;
+      const int h0 = (u - t * chunks) * S * R + sub;
+      const T* x = static_cast<const T*>(sd.x) + t * sd.x_row + i;
+      const T* g = static_cast<const T*>(sd.g) + t * sd.g_row + i;
+      uint4 xr[R], gr[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int h = h0 + r * S;
+        const bool in = active && h < sd.heads;
+        xr[r] = in ? *reinterpret_cast<const uint4*>(x + h * sd.x_head) : make_uint4(0, 0, 0, 0);
+        gr[r] = in ? *reinterpret_cast<const uint4*>(g + h * sd.g_head) : make_uint4(0, 0, 0, 0);
+      }
+      const long long pos = qk_position(args, t);
+      if (pos < 0 || pos >= args.table_rows) {
+        if (lane == 0) report_status(kStatusBadPosition, t);
+        continue;
+      }
+      QkAngles ang = {};
+      if (turns) qk_load_angles<PAIRS>(args.cos_sin + pos * args.rot, args.rot, i, ang);
+      T* out = static_cast<T*>(sd.out) + t * sd.out_row + i;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int h = h0 + r * S;
+        float v[8], gv[8], ss = 0.f, dot = 0.f;
+        qk_unpack<T>(xr[r], v);
+        qk_unpack<T>(gr[r], gv);
+        qk_rotate<PAIRS>(gv, ang, turns, partner, -1.f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+        const float rs = rsqrtf(fmaf(qk_row_sum<L>(ss), inv_dim, args.eps));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[j] *= rs;                          // n
+          dw[j] = fmaf(gv[j], v[j], dw[j]);
+          gv[j] *= w[j];
+          dot = fmaf(gv[j], v[j], dot);
+        }
+        const float mean = qk_row_sum<L>(dot) * inv_dim;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) gv[j] = rs * (gv[j] - v[j] * mean);
+        if (active && h < sd.heads)
+          *reinterpret_cast<uint4*>(out + h * sd.out_head) = qk_pack<T>(gv);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sums[warp * S + sub][i + j] = dw[j];
+    __syncthreads();
+    for (int d = threadIdx.x; d < args.dim; d += kQkThreads) {
+      float total = 0.f;
+#pragma unroll
+      for (int r = 0; r < kQkWarps * S; ++r) total += sums[r][d];
+      args.partials[(static_cast<size_t>(blockIdx.x) * 2 + side) * args.dim + d] = total;
+    }
+    __syncthreads();
+  }
+}
+
+// Any head size up to kQkMaxDim, any even rot, any strides: one warp per head
+// row, the row staged in shared memory in fp32.  Blocks are persistent in both
+// directions; the weight gradient is accumulated per warp in shared memory
+// (each lane owns its columns).
+template <typename T, bool PAIRS, bool GRAD>
+__global__ void __launch_bounds__(128) qk_norm_rope_any_kernel(const QkArgs args) {
+  extern __shared__ float rows[];  // [4 warps][3][dim]: x, gradient, weight gradient
+  pdl_allow_next();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int D = args.dim, hr = args.rot / 2;
+  const float inv_dim = 1.f / D;
+  float* v = rows + static_cast<size_t>(warp) * 3 * D;
+  float* gv = v + D;
+  float* dw = gv + D;
+  pdl_wait();
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    const QkSide& sd = args.side[side];
+    const T* w = static_cast<const T*>(sd.w);
+    const int units = args.tokens * sd.heads;
+    if (GRAD)
+      for (int d = lane; d < D; d += 32) dw[d] = 0.f;
+    for (int u = blockIdx.x * 4 + warp; u < units; u += gridDim.x * 4) {
+      const int t = u / sd.heads, h = u - t * sd.heads;
+      const long long pos = qk_position(args, t);
+      if (pos < 0 || pos >= args.table_rows) {
+        if (lane == 0) report_status(kStatusBadPosition, t);
+        continue;
+      }
+      const float* cs = args.cos_sin + pos * args.rot;
+      const T* x = static_cast<const T*>(sd.x) + t * sd.x_row + h * sd.x_head;
+      T* out = static_cast<T*>(sd.out) + t * sd.out_row + h * sd.out_head;
+      float ss = 0.f;
+      for (int d = lane; d < D; d += 32) {
+        const float f = Pack2<T>::to_float(x[d]);
+        v[d] = f;
+        ss = fmaf(f, f, ss);
+        if (GRAD)
+          gv[d] = Pack2<T>::to_float(static_cast<const T*>(sd.g)[t * sd.g_row + h * sd.g_head + d]);
+      }
+      const float rs = rsqrtf(fmaf(qk_row_sum<32>(ss), inv_dim, args.eps));
+      __syncwarp();
+      if (!GRAD) {
+        for (int d = lane; d < D; d += 32) v[d] = v[d] * rs * Pack2<T>::to_float(w[d]);
+        __syncwarp();
+      }
+      float* y = GRAD ? gv : v;
+      for (int p = lane; p < hr; p += 32) {
+        const int a = PAIRS ? 2 * p : p, b = PAIRS ? 2 * p + 1 : p + hr;
+        const float c = cs[p], s = GRAD ? -cs[hr + p] : cs[hr + p];
+        const float ya = y[a], yb = y[b];
+        y[a] = fmaf(ya, c, -(yb * s));
+        y[b] = fmaf(yb, c, ya * s);
+      }
+      __syncwarp();
+      if (GRAD) {
+        float dot = 0.f;
+        for (int d = lane; d < D; d += 32) {
+          const float n = v[d] * rs, g = gv[d];
+          dw[d] = fmaf(g, n, dw[d]);
+          dot = fmaf(g * Pack2<T>::to_float(w[d]), n, dot);
+        }
+        const float mean = qk_row_sum<32>(dot) * inv_dim;
+        for (int d = lane; d < D; d += 32)
+          out[d] = Pack2<T>::from_float(
+              rs * (gv[d] * Pack2<T>::to_float(w[d]) - v[d] * rs * mean));
+      } else {
+        for (int d = lane; d < D; d += 32) out[d] = Pack2<T>::from_float(v[d]);
+      }
+      __syncwarp();
+    }
+    if (GRAD) {
+      __syncthreads();
+      for (int d = threadIdx.x; d < D; d += 128) {
+        float total = 0.f;
+        for (int r = 0; r < 4; ++r) total += rows[(r * 3 + 2) * static_cast<size_t>(D) + d];
+        args.partials[(static_cast<size_t>(blockIdx.x) * 2 + side) * D + d] = total;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// dw[side][d] = sum over blocks of the partial rows, in a fixed order: thread
+// (x, y) adds blocks y, y + 32, ..., then the 32 sums of a column are added in
+// y order.
+__global__ void __launch_bounds__(1024) qk_norm_rope_dweight_kernel(const float* partials,
+                                                                    int blocks, int dim,
+                                                                    float* dqw, float* dkw) {
+  __shared__ float part[32][33];
+  pdl_allow_next();
+  pdl_wait();
+  const int side = blockIdx.y, d = blockIdx.x * 32 + threadIdx.x;
+  float sum = 0.f;
+  if (d < dim)
+    for (int b = threadIdx.y; b < blocks; b += 32)
+      sum += partials[(static_cast<size_t>(b) * 2 + side) * dim + d];
+  part[threadIdx.y][threadIdx.x] = sum;
+  __syncthreads();
+  if (threadIdx.y == 0 && d < dim) {
+    float total = 0.f;
+#pragma unroll
+    for (int y = 0; y < 32; ++y) total += part[y][threadIdx.x];
+    (side ? dkw : dqw)[d] = total;
+  }
+}
+
+// cos_sin[p][i] = cos(p base^(-2 i / rot)), cos_sin[p][rot / 2 + i] = its sine;
+// angles in 64 bits (fp32 has no correct digit of the sine left once the angle
+// passes 2^24), rounded once to fp32.
+__global__ void __launch_bounds__(256) rope_table_kernel(float* cos_sin, int rows, int rot,
+                                                         double base) {
+  pdl_allow_next();
+  pdl_wait();
+  const int hr = rot / 2;
+  const int64_t n = static_cast<int64_t>(rows) * hr;
+  for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < n; e += gridDim.x * 256ll) {
+    const int64_t p = e / hr;
+    const int i = static_cast<int>(e - p * hr);
+    double sn, cn;
+    sincos(static_cast<double>(p) * pow(base, -2.0 * i / rot), &sn, &cn);
+    cos_sin[p * rot + i] = static_cast<float>(cn);
+    cos_sin[p * rot + hr + i] = static_cast<float>(sn);
+  }
+}
+
+}  // namespace bokt

@@ -208,6 +208,55 @@ int bokt_rmsnorm_gemm(const void* X, const void* B_folded, void* C, float* row_s
                       void* stream);
 
 /*
+ * RMSNorm of every query and key head and the rotary position rotation in one
+ * pass.  q [tokens, heads, dim] and k [tokens, kv_heads, dim] are views with
+ * element strides (last dimension contiguous), as the projection leaves them
+ * side by side; per head x:
+ *   y = x * rsqrt(mean(x^2) + eps) * w,   then y[:rot] turned by the angle of
+ * positions[t] (int32, or int64 with positions_i64): for i < rot / 2 the pair
+ * (i, i + rot / 2), or (2 i, 2 i + 1) with interleaved, turns by the angle
+ * whose cosine is cos_sin[p][i] and whose sine is cos_sin[p][rot / 2 + i]
+ * (fp32 [table_rows, rot]).  fp32 arithmetic, one rounding.  q_out / k_out may
+ * be q / k themselves (same strides).  A position outside the table sets the
+ * device status word (code 5) and leaves that token's heads unwritten.
+ * strides[8]: q row, q head, q_out row, q_out head, then the same of k.
+ * dim in [2, 1024], rot even; dim a multiple of 8 up to 256 with 16-byte
+ * aligned rows and rot a multiple of 16 (8 interleaved) runs vectorised.  The
+ * RMSNorm of kernels/rmsnorm.py:22-25 applied to each head; the rotation has
+ * no counterpart in the reference.
+ */
+int bokt_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                      const void* positions, int positions_i64, const float* cos_sin,
+                      int table_rows, void* q_out, void* k_out, int tokens, int heads,
+                      int kv_heads, int dim, int rot, const int64_t* strides, int interleaved,
+                      float eps, int dtype, void* stream);
+
+/*
+ * Gradients of bokt_qk_norm_rope: dq, dk (may be dq_out / dk_out themselves)
+ * and the weights' gradients dq_weight, dk_weight (fp32 [dim], overwritten;
+ * summed in a fixed order for a given device and shape).  The row statistics
+ * are recomputed from q and k.  strides[12]: q row, q head, dq row, dq head,
+ * dq_out row, dq_out head, then the same of k.  A token whose position is
+ * outside the table contributes nothing and its dq / dk rows are left
+ * unwritten.  workspace: bokt_qk_norm_rope_workspace_bytes(dim) bytes of
+ * device scratch, contents free before and after (-1: no usable device).
+ */
+int64_t bokt_qk_norm_rope_workspace_bytes(int dim);
+int bokt_qk_norm_rope_backward(const void* dq_out, const void* dk_out, const void* q,
+                               const void* k, const void* q_weight, const void* k_weight,
+                               const void* positions, int positions_i64, const float* cos_sin,
+                               int table_rows, void* dq, void* dk, float* dq_weight,
+                               float* dk_weight, int tokens, int heads, int kv_heads, int dim,
+                               int rot, const int64_t* strides, int interleaved, float eps,
+                               int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * cos_sin[p][i] = cos(p * base^(-2 i / rot)), cos_sin[p][rot / 2 + i] its sine
+ * for p < rows, i < rot / 2; angles in 64 bits, rounded once to fp32.
+ */
+int bokt_rope_table(float* cos_sin, int rows, int rot, double base, void* stream);
+
+/*
  * For each expert e: Y[off[e]:off[e+1]] = X[off[e]:off[e+1]] * W[e], W of shape
  * [E,K,N]; X and Y have T rows.  offsets has E+1 entries, int32
  * (offsets_is_i64 = 0) or int64 (1), resident on the device and read by the
