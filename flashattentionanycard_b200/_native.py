@@ -5,6 +5,7 @@ fallback behind the ``launch`` functions.  A missing or stale library raises
 ``RuntimeError`` at the first call instead of silently running something else.
 """
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -198,9 +199,24 @@ def dtype_code(dtype):
 
 
 def current_stream(device):
+    """Handle of torch's current stream on a tensor's device (without building
+    the Stream object, which costs more than a decode kernel runs)."""
     import torch
 
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context in which ``device`` (a tensor's) is the current CUDA device; the
+    library launches on the current one.  Free of cost where it already is."""
+    import torch
+
+    if torch.cuda.current_device() == device.index:
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
 
 
 def device_status(reset=True):

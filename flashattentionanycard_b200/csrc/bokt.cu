@@ -1501,8 +1501,14 @@ cudaError_t launch_qk_any(const bokt::QkArgs& a, int sm_count, int* blocks, cuda
 }
 
 template <typename T, int L, bool PAIRS, int R, bool GRAD>
-cudaError_t launch_qk_vec(const bokt::QkArgs& a, int sm_count, int* blocks, cudaStream_t s) {
-  constexpr int hpu = 32 / L * R;
+cudaError_t launch_qk_vec(bokt::QkArgs a, int sm_count, int* blocks, cudaStream_t s) {
+  // As many rows behind one load of the angles as leave every SM two rounds
+  // of 32 warps, up to the measured best (four loops forward, two backward).
+  const long long rows = (long long)a.tokens * (a.side[0].heads + a.side[1].heads);
+  a.loops = 1;
+  while (R > 1 && a.loops < (GRAD ? 2 : 4) && rows / (32 / L * R * 2 * a.loops) >= 64ll * sm_count)
+    a.loops *= 2;
+  const int hpu = 32 / L * R * a.loops;
   const long long u0 = (long long)a.tokens * ((a.side[0].heads + hpu - 1) / hpu);
   const long long u1 = (long long)a.tokens * ((a.side[1].heads + hpu - 1) / hpu);
   if constexpr (GRAD) {
@@ -1524,7 +1530,7 @@ template <typename T, bool PAIRS, bool GRAD>
 cudaError_t launch_qk(const bokt::QkArgs& a, bool vec, int sm_count, int* blocks, cudaStream_t s) {
   if (!vec) return launch_qk_any<T, PAIRS, GRAD>(a, sm_count, blocks, s);
   // Few head rows: one row per lane group, so that the call spreads over the
-  // SMs; many: four rows share a token's angles and keep four loads in flight.
+  // SMs; many: four loads in flight per lane.
   const bool few = (long long)a.tokens * (a.side[0].heads + a.side[1].heads) < 64ll * sm_count;
 #define BOKT_QK(L) \
   (few ? launch_qk_vec<T, L, PAIRS, 1, GRAD>(a, sm_count, blocks, s) \

@@ -34,7 +34,7 @@ def rope_table(rows, rot, base=10000.0, device="cuda"):
     if not (math.isfinite(base) and base > 0):
         raise ValueError("base must be finite and positive")
     out = torch.empty((rows, rot), device=device, dtype=torch.float32)
-    with torch.cuda.device(out.device):
+    with _native.on_device(out.device):
         _native.check(
             _native.load().bokt_rope_table(out.data_ptr(), rows, rot, float(base),
                                            _native.current_stream(out.device)),
@@ -43,17 +43,10 @@ def rope_table(rows, rot, base=10000.0, device="cuda"):
     return out
 
 
-def _writable(t, name):
-    """Distinct elements of an output view must be distinct memory."""
-    spans = sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1)
-    reach = 0
-    for stride, n in spans:
-        if stride <= reach:
-            raise ValueError(f"{name} must not overlap itself (strides {t.stride()})")
-        reach += stride * (n - 1)
-
-
 def _check(named, q, k, positions, cos_sin, weights, epsilon, writes):
+    """Shapes, types, layouts and devices of a call; returns (tokens, head size, rot).
+
+    Decode calls are shorter than these checks, so each is a plain comparison."""
     import torch
 
     if q.dim() != 3 or k.dim() != 3:
@@ -61,24 +54,27 @@ def _check(named, q, k, positions, cos_sin, weights, epsilon, writes):
     t, _, d = q.shape
     if k.shape[0] != t or k.shape[2] != d:
         raise ValueError(f"shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}")
-    for name, (tensor, like) in named.items():
-        if tensor.shape != like.shape:
-            raise ValueError(f"shape mismatch: {name} {tuple(tensor.shape)}, expected {tuple(like.shape)}")
-    views = {"q": q, "k": k, **{n: v for n, (v, _) in named.items()}}
-    for name, v in views.items():
-        if v.dtype != q.dtype:
+    dtype, device = q.dtype, q.device
+    for name, x, like in named:
+        if x.shape != like.shape:
+            raise ValueError(f"shape mismatch: {name} {tuple(x.shape)}, expected {tuple(like.shape)}")
+        if x.dtype != dtype:
             raise ValueError(f"{name} must share q's dtype")
-        if d > 1 and v.stride(2) != 1:
+        row, head, last = x.stride()
+        if last != 1 and d > 1:
             raise ValueError(f"{name} must be contiguous in its last dimension")
-    for name in writes:
-        _writable(views[name], name)
-    for name, w in weights.items():
-        if tuple(w.shape) != (d,) or not w.is_contiguous():
+        if name in writes:
+            # Distinct elements of an output must be distinct memory.
+            n, h, _ = x.shape
+            if not (n * h <= 1 or (n == 1 and head >= d) or (h == 1 and row >= d)
+                    or (head >= d and row >= head * (h - 1) + d) or (row >= d and head >= row * (n - 1) + d)):
+                raise ValueError(f"{name} must not overlap itself (strides {x.stride()})")
+    for name, w, wtype in weights:
+        if w.shape != (d,) or not w.is_contiguous():
             raise ValueError(f"{name} must be a contiguous tensor of {d} elements")
-    for name in ("q_weight", "k_weight"):
-        if weights[name].dtype != q.dtype:
-            raise ValueError(f"{name} must share q's dtype")
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (t,) \
+        if w.dtype != (wtype or dtype):
+            raise ValueError(f"{name} must " + ("be fp32" if wtype else "share q's dtype"))
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (t,) \
             or not positions.is_contiguous():
         raise ValueError(f"positions must be a contiguous int32 or int64 tensor of {t} elements")
     if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
@@ -88,22 +84,23 @@ def _check(named, q, k, positions, cos_sin, weights, epsilon, writes):
         raise ValueError(f"rot (cos_sin's width) must be even and in [2, {d}], got {rot}")
     if not (math.isfinite(epsilon) and epsilon >= 0):
         raise ValueError("epsilon must be finite and non-negative")
-    tensors = [*views.values(), *weights.values(), positions, cos_sin]
-    if not all(x.is_cuda for x in tensors) or len({x.device for x in tensors}) != 1:
+    if not (q.is_cuda and positions.device == device and cos_sin.device == device
+            and all(x.device == device for _, x, _ in named) and all(w.device == device for _, w, _ in weights)):
         raise ValueError("all tensors must be on one CUDA device")
     return t, d, rot
 
 
 def launch(q, k, q_weight, k_weight, positions, cos_sin, q_out, k_out, epsilon=1e-6, interleaved=False):
     """q_out, k_out = rotated norms of q's and k's heads (q_out may be q, k_out may be k)."""
-    t, d, rot = _check({"q_out": (q_out, q), "k_out": (k_out, k)}, q, k, positions, cos_sin,
-                       {"q_weight": q_weight, "k_weight": k_weight}, epsilon, ("q_out", "k_out"))
     import torch
 
+    t, d, rot = _check((("q", q, q), ("k", k, k), ("q_out", q_out, q), ("k_out", k_out, k)), q, k,
+                       positions, cos_sin, (("q_weight", q_weight, None), ("k_weight", k_weight, None)),
+                       epsilon, ("q_out", "k_out"))
     lib = _native.load()
     strides = (ctypes.c_int64 * 8)(q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1),
                                    k.stride(0), k.stride(1), k_out.stride(0), k_out.stride(1))
-    with torch.cuda.device(q.device):
+    with _native.on_device(q.device):
         _native.check(
             lib.bokt_qk_norm_rope(
                 q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
@@ -123,18 +120,17 @@ def launch_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, cos_sin
     order: the same inputs give the same bits)."""
     import torch
 
-    if dq_weight.dtype != torch.float32 or dk_weight.dtype != torch.float32:
-        raise ValueError("dq_weight and dk_weight must be fp32")
-    t, d, rot = _check({"dq_out": (dq_out, q), "dk_out": (dk_out, k), "dq": (dq, q), "dk": (dk, k)},
-                       q, k, positions, cos_sin,
-                       {"q_weight": q_weight, "k_weight": k_weight, "dq_weight": dq_weight,
-                        "dk_weight": dk_weight}, epsilon, ("dq", "dk"))
+    t, d, rot = _check(
+        (("q", q, q), ("k", k, k), ("dq_out", dq_out, q), ("dk_out", dk_out, k), ("dq", dq, q), ("dk", dk, k)),
+        q, k, positions, cos_sin,
+        (("q_weight", q_weight, None), ("k_weight", k_weight, None), ("dq_weight", dq_weight, torch.float32),
+         ("dk_weight", dk_weight, torch.float32)), epsilon, ("dq", "dk"))
     lib = _native.load()
     strides = (ctypes.c_int64 * 12)()
     for i, (x, dx, g) in enumerate(((q, dq, dq_out), (k, dk, dk_out))):
         strides[6 * i:6 * i + 6] = [x.stride(0), x.stride(1), dx.stride(0), dx.stride(1), g.stride(0),
                                     g.stride(1)]
-    with torch.cuda.device(q.device):
+    with _native.on_device(q.device):
         nbytes = int(lib.bokt_qk_norm_rope_workspace_bytes(d))
         if nbytes < 0:
             _native.check(_native.BOKT_ERR_CUDA_RC, "bokt_qk_norm_rope_workspace_bytes")
