@@ -131,6 +131,8 @@ SIGNATURES = {
     "bokt_selftest_bounded_wait": (_I32, [_I64, _VP, _VP]),
     "bokt_moe_topk_gate": (_I32, [_VP, _I32, _I32, _I32, _I32, _I32, _VP, _VP, _VP]),
     "bokt_moe_combine": (_I32, [_VP, _I64, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _VP]),
+    "bokt_moe_decode_workspace_bytes": (_I64, [_I32] * 5),
+    "bokt_moe_decode": (_I32, [_VP, _VP, _I32, _VP, _VP, _VP] + [_I32] * 7 + [_VP, _I64, _VP]),
     "bokt_kernel_attrs": (
         _I32,
         [_I32, _I32, _I32, _I32, _PP, ctypes.POINTER(BoktAttrs)],
@@ -203,7 +205,8 @@ def current_stream(device):
     the Stream object, which costs more than a decode kernel runs)."""
     import torch
 
-    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(device.index))
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
 
 
 _SAME_DEVICE = contextlib.nullcontext()

@@ -16,6 +16,7 @@
 #include "gemm_edge.cuh"
 #include "gemm_tc.cuh"
 #include "gemm_tc2.cuh"
+#include "moe_decode.cuh"
 #include "moe_route.cuh"
 #include "norm_gemm.cuh"
 #include "qk_norm_rope.cuh"
@@ -1661,6 +1662,184 @@ int bokt_rope_table(float* cos_sin, int rows, int rot, double base, void* stream
   cudaError_t e = launch(bokt::rope_table_kernel, dim3(unsigned(blocks)), dim3(256), 0,
                          static_cast<cudaStream_t>(stream), cos_sin, rows, rot, base);
   if (e != cudaSuccess) return cuda_fail(e, "rope_table launch");
+  return BOKT_OK;
+}
+
+}  // extern "C"
+
+// ----------------------------------------------------------------- MoE layer for a few tokens
+namespace {
+
+// Byte offsets of the workspace's parts, each 256-byte aligned.
+struct MoeDecodeLayout {
+  int shares;
+  int64_t act_e, act_off, row_token, row_of, act_of, gates, h, y, part, total;
+};
+
+int moe_decode_layout(int tokens, int E, int K, int I, int topk, const DeviceInfo& dev,
+                      MoeDecodeLayout* l) {
+  if (tokens < 0 || E <= 0 || K <= 0 || I <= 0 || topk <= 0)
+    return fail(BOKT_ERR_INVALID, "need tokens >= 0 and positive sizes");
+  if (topk > E) return fail(BOKT_ERR_INVALID, "topk %d exceeds the %d experts", topk, E);
+  if (tokens > bokt::kMdMaxTokens || topk > bokt::kMdMaxTopk || E > bokt::kMdMaxExperts)
+    return fail(BOKT_ERR_UNSUPPORTED,
+                "at most %d tokens, top-%d and %d experts (got %d, %d, %d); route more tokens "
+                "through bokt_moe_route and bokt_moe_grouped_gemm", bokt::kMdMaxTokens,
+                bokt::kMdMaxTopk, bokt::kMdMaxExperts, tokens, topk, E);
+  if (K % 8 != 0 || I % 8 != 0 || K > 65536 || I > 65536)
+    return fail(BOKT_ERR_UNSUPPORTED, "K and I must be multiples of 8 up to 65536 (got %d, %d)", K, I);
+  // Every share holds at least one k-step of either phase: topk experts are in use at least.
+  const long long u1 = (long long)topk * ((I + 127) / 128) * ((K + 63) / 64);
+  const long long u2 = (long long)topk * ((K + 255) / 256) * ((I + 63) / 64);
+  long long g = dev.sm_count;
+  if (u1 < g) g = u1;
+  if (u2 < g) g = u2;
+  l->shares = int(g);
+  const int64_t A = (int64_t)tokens * topk, em = E < A ? E : A;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t r = at;
+    at += (bytes + 255) / 256 * 256;
+    return r;
+  };
+  take((bokt::kMdCount1 + 4 * g) * 4);
+  l->act_e = take(em * 4);
+  l->act_off = take((em + 1) * 4);
+  l->row_token = take(A * 4);
+  l->row_of = take(A * 4);
+  l->act_of = take(A * 4);
+  l->gates = take(A * 4);
+  l->h = take(A * I * 2);
+  l->y = take(A * K * 4);
+  l->part = take(2 * g * tokens * 256 * 4);
+  l->total = at;
+  return BOKT_OK;
+}
+
+template <typename LT>
+const void* moe_decode_gate_ptr(int E) {
+  if (E <= 32) return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<LT, 1>);
+  if (E <= 128) return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<LT, 4>);
+  if (E <= 256) return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<LT, 8>);
+  return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<LT, 32>);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t bokt_moe_decode_workspace_bytes(int tokens, int E, int K, int I, int topk) {
+  g_err[0] = 0;
+  DeviceInfo dev;
+  MoeDecodeLayout l;
+  if (device_info(&dev) || moe_decode_layout(tokens, E, K, I, topk, dev, &l)) return -1;
+  return l.total;
+}
+
+int bokt_moe_decode(const void* x, const void* logits, int logits_dtype, const void* w_gate_up,
+                    const void* w_down, void* out, int tokens, int E, int K, int I, int topk,
+                    int renormalize, int dtype, void* workspace, int64_t workspace_bytes,
+                    void* stream) {
+  g_err[0] = 0;
+  if (dtype != BOKT_FP16 && dtype != BOKT_BF16) return fail(BOKT_ERR_INVALID, "dtype %d", dtype);
+  if (logits_dtype != BOKT_FP16 && logits_dtype != BOKT_BF16 && logits_dtype != BOKT_FP32)
+    return fail(BOKT_ERR_INVALID, "logits dtype %d", logits_dtype);
+  DeviceInfo dev = {};
+  MoeDecodeLayout l;
+  int rc = moe_decode_layout(tokens, E, K, I, topk, dev, &l);  // sizes, before any device call
+  if (rc) return rc;
+  if (tokens == 0) return BOKT_OK;
+  if (!x || !logits || !w_gate_up || !w_down || !out || !workspace)
+    return fail(BOKT_ERR_INVALID, "null pointer");
+  if (!aligned16(x) || !aligned16(w_gate_up) || !aligned16(w_down) || !aligned16(out))
+    return fail(BOKT_ERR_UNSUPPORTED, "x, weights and out must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(BOKT_ERR_INVALID, "workspace must be 256-byte aligned");
+  rc = device_info(&dev);
+  if (rc) return rc;
+  rc = moe_decode_layout(tokens, E, K, I, topk, dev, &l);
+  if (rc) return rc;
+  if (workspace_bytes < l.total)
+    return fail(BOKT_ERR_INVALID, "workspace too small: %lld bytes, need %lld",
+                (long long)workspace_bytes, (long long)l.total);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int A = tokens * topk;
+  bokt::MoeDecodeArgs a = {};
+  a.tokens = tokens, a.experts = E, a.k = K, a.inner = I, a.topk = topk;
+  a.nt = (tokens + 15) & ~15;
+  a.shares = l.shares;
+  a.idesc = bokt::make_idesc_f16_swapped(uint32_t(dtype), 0);
+  a.header = reinterpret_cast<uint32_t*>(ws);
+  a.act_e = reinterpret_cast<int*>(ws + l.act_e);
+  a.act_off = reinterpret_cast<int*>(ws + l.act_off);
+  a.row_token = reinterpret_cast<int*>(ws + l.row_token);
+  a.row_of = reinterpret_cast<int*>(ws + l.row_of);
+  a.act_of = reinterpret_cast<int*>(ws + l.act_of);
+  a.gates = reinterpret_cast<float*>(ws + l.gates);
+  a.h = ws + l.h;
+  a.y = reinterpret_cast<float*>(ws + l.y);
+  a.part = reinterpret_cast<float*>(ws + l.part);
+  a.out = out;
+  const int emax = E < A ? E : A;
+  a.stages = bokt::kMdMaxStages;
+  while (a.stages > 2 && bokt::moe_decode_smem_bytes(a.nt, a.stages, emax, A) > dev.smem_optin)
+    --a.stages;
+  int smem = bokt::moe_decode_smem_bytes(a.nt, a.stages, emax, A);
+  if (smem > dev.smem_optin) return fail(BOKT_ERR_UNSUPPORTED, "needs %d bytes of shared memory", smem);
+  // One CTA per SM (its TMEM may be all 512 columns).
+  if (smem < dev.smem_optin / 2 + 1024) smem = dev.smem_optin / 2 + 1024;
+
+  const bool fp16 = dtype == BOKT_FP16;
+  CUtensorMap mg, md, mx, mh;
+  {
+    const uint64_t d[3] = {uint64_t(2) * I, uint64_t(K), uint64_t(E)};
+    const uint64_t st[2] = {uint64_t(I) * 4, uint64_t(I) * 4 * K};
+    const uint32_t b[3] = {64, 64, 1};
+    if ((rc = encode_map(&mg, w_gate_up, 3, d, st, b, fp16))) return rc;
+  }
+  {
+    const uint64_t d[3] = {uint64_t(K), uint64_t(I), uint64_t(E)};
+    const uint64_t st[2] = {uint64_t(K) * 2, uint64_t(K) * 2 * I};
+    const uint32_t b[3] = {64, 64, 1};
+    if ((rc = encode_map(&md, w_down, 3, d, st, b, fp16))) return rc;
+  }
+  {
+    const uint64_t d[2] = {uint64_t(K), uint64_t(tokens)};
+    const uint64_t st[1] = {uint64_t(K) * 2};
+    const uint32_t b[2] = {64, uint32_t(a.nt)};
+    if ((rc = encode_map(&mx, x, 2, d, st, b, fp16))) return rc;
+  }
+  {
+    const uint64_t d[2] = {uint64_t(I), uint64_t(A)};
+    const uint64_t st[1] = {uint64_t(I) * 2};
+    const uint32_t b[2] = {64, 16};
+    if ((rc = encode_map(&mh, a.h, 2, d, st, b, fp16))) return rc;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  {
+    const void* fn = logits_dtype == BOKT_FP32 ? moe_decode_gate_ptr<float>(E)
+                     : logits_dtype == BOKT_BF16 ? moe_decode_gate_ptr<__nv_bfloat16>(E)
+                                                 : moe_decode_gate_ptr<__half>(E);
+    const unsigned ctas = unsigned((tokens + 31) / 32);
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t lc = launch_config(dim3(ctas), dim3(1024), 0, s, attr);
+    attr[lc.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[lc.numAttrs].val.clusterDim.x = ctas;
+    attr[lc.numAttrs].val.clusterDim.y = 1;
+    attr[lc.numAttrs].val.clusterDim.z = 1;
+    lc.numAttrs += 1;
+    int renorm = renormalize ? 1 : 0;
+    void* kargs[] = {const_cast<void*>(static_cast<const void*>(&logits)), &renorm, &a};
+    cudaError_t e = cudaLaunchKernelExC(&lc, fn, kargs);
+    if (e != cudaSuccess) return cuda_fail(e, "moe_decode_gate launch");
+  }
+  const void* fn = dtype == BOKT_BF16
+                       ? reinterpret_cast<const void*>(&bokt::moe_decode_kernel<__nv_bfloat16>)
+                       : reinterpret_cast<const void*>(&bokt::moe_decode_kernel<__half>);
+  if ((rc = ensure_smem(fn, smem))) return rc;
+  void* kargs[] = {&mg, &md, &mx, &mh, &a};
+  cudaError_t e = launch_ptr(fn, dim3(unsigned(a.shares)), dim3(bokt::kMdThreads), smem, s, kargs);
+  if (e != cudaSuccess) return cuda_fail(e, "moe_decode launch");
   return BOKT_OK;
 }
 

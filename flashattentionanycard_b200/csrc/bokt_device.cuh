@@ -245,6 +245,13 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(uint32_t ab_format, uint32
          ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
+// The same with A MN-major and B K-major (weights as the 128-row operand,
+// tokens as the narrow one); n may be left 0 and joined per tile.
+__host__ __device__ constexpr uint32_t make_idesc_f16_swapped(uint32_t ab_format, uint32_t n) {
+  return (1u << 4) | (ab_format << 7) | (ab_format << 10) | (1u << 15) | (0u << 16) |
+         ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
 // ---------------------------------------------------------------------------
 // Element conversion helpers.
 // ---------------------------------------------------------------------------

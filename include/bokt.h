@@ -492,6 +492,31 @@ int bokt_moe_combine(const void* y, int64_t y_rows, const int32_t* rows, const f
                      void* out, int tokens, int k, int N, int dtype, void* stream);
 
 /*
+ * A whole mixture-of-experts layer for a few tokens, two kernels: per token
+ *   p = softmax(logits[t]) (fp32), the topk largest (ties to the lower index)
+ *   with gates p, divided by their sum when renormalize != 0,
+ *   out[t] = sum_j gate_j (silu(x[t] Wg_j) * (x[t] Wu_j)) Wd_j
+ * with [Wg | Wu] = w_gate_up[e] ([K, 2 I]) and Wd = w_down[e] ([I, K]).  The
+ * weights of every expert in use are read once.  silu(gate) * up is rounded to
+ * dtype (it is a tensor-core operand); the experts' results are summed in fp32
+ * and rounded once.  x, out [tokens, K]; logits [tokens, E] fp16/bf16/fp32.
+ * A NaN logit makes its token's gates and output NaN.  tokens <= 128,
+ * topk <= 8, E <= 1024, K and I multiples of 8, 16-byte aligned pointers (else
+ * BOKT_ERR_UNSUPPORTED: larger batches go through bokt_moe_topk_gate,
+ * bokt_moe_route and bokt_moe_grouped_gemm).  workspace:
+ * bokt_moe_decode_workspace_bytes(...) bytes of device scratch, 256-byte
+ * aligned, contents free before and after; calls that overlap on the GPU need
+ * one each.  No counterpart in the reference, which has the grouped product of
+ * one projection (kernels/moe_grouped_gemm.py:11-58) and leaves gate, routing,
+ * activation and combine to the caller.
+ */
+int64_t bokt_moe_decode_workspace_bytes(int tokens, int E, int K, int I, int topk);
+int bokt_moe_decode(const void* x, const void* logits, int logits_dtype, const void* w_gate_up,
+                    const void* w_down, void* out, int tokens, int E, int K, int I, int topk,
+                    int renormalize, int dtype, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
+/*
  * Failure-detection self-test: launches one CTA that waits on an mbarrier
  * nothing will complete, with the same bounded wait every pipelined kernel
  * uses.  After timeout_ns (<= 10 s) the wait gives up, the kernel writes 1 to
