@@ -1688,13 +1688,8 @@ int moe_decode_layout(int tokens, int E, int K, int I, int topk, const DeviceInf
                 bokt::kMdMaxTopk, bokt::kMdMaxExperts, tokens, topk, E);
   if (K % 8 != 0 || I % 8 != 0 || K > 65536 || I > 65536)
     return fail(BOKT_ERR_UNSUPPORTED, "K and I must be multiples of 8 up to 65536 (got %d, %d)", K, I);
-  // Every share holds at least one k-step of either phase: topk experts are in use at least.
-  const long long u1 = (long long)topk * ((I + 127) / 128) * ((K + 63) / 64);
-  const long long u2 = (long long)topk * ((K + 255) / 256) * ((I + 63) / 64);
-  long long g = dev.sm_count;
-  if (u1 < g) g = u1;
-  if (u2 < g) g = u2;
-  l->shares = int(g);
+  const int64_t g = dev.sm_count;
+  l->shares = dev.sm_count;
   const int64_t A = (int64_t)tokens * topk, em = E < A ? E : A;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {

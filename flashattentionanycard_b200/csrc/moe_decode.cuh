@@ -49,6 +49,10 @@ constexpr int kMdMaxExperts = 1024;
 constexpr int kMdStageW = 32768;  // 4 boxes of 64 columns x 64 k
 constexpr int kMdQueue = 4;
 constexpr int kMdMaxStages = 8;
+// Fewest k-steps of a share: below that a tile's partial sums cost more than the
+// spreading saves (one token, 8 experts x [1024, 2 x 2048]: 29.2 us a call with 1,
+// 24.2 with 4, 25.8 with 8).
+constexpr int kMdMinSteps = 4;
 
 // Header words of the workspace.
 constexpr int kMdClaim = 0, kMdDone1 = 32, kMdDone2 = 64, kMdActive = 96, kMdCount1 = 128;
@@ -254,20 +258,32 @@ __device__ __forceinline__ int md_share_of(int u, int units, int shares) {
 }
 
 struct MdPlan {
-  int active;              // experts in use
-  int tiles1, steps1, units1;  // per expert: tiles1 of 128 + 128 columns
-  int tiles2, steps2, units2;  // tiles2 column blocks of 256, experts inside
+  int active;                          // experts in use
+  int tiles1, steps1, units1, shares1;  // per expert: tiles1 of 128 + 128 columns
+  int tiles2, steps2, units2, shares2;  // tiles2 column blocks of 256, experts inside
+  int claims;                          // of all phases
   const int* act_e;
   const int* act_off;
   const int* row_token;
 };
 
-__device__ __forceinline__ MdSegments md_segments(const MdPlan& p, int claim, int shares, int* phase) {
+// Phase (0, 1, 2) of a claim; *share: its share of that phase.
+__device__ __forceinline__ int md_phase(const MdPlan& p, int claim, int* share) {
+  if (claim < p.shares1) {
+    *share = claim;
+    return 0;
+  }
+  claim -= p.shares1;
+  const int phase = claim < p.shares2 ? 1 : 2;
+  *share = phase == 1 ? claim : claim - p.shares2;
+  return phase;
+}
+
+__device__ __forceinline__ MdSegments md_segments(const MdPlan& p, int phase, int share) {
   MdSegments s;
-  *phase = claim / shares;
-  const int share = claim - *phase * shares;
-  const int units = *phase == 0 ? p.units1 : p.units2;
-  s.steps = *phase == 0 ? p.steps1 : p.steps2;
+  const int units = phase == 0 ? p.units1 : p.units2;
+  const int shares = phase == 0 ? p.shares1 : p.shares2;
+  s.steps = phase == 0 ? p.steps1 : p.steps2;
   s.u = md_share_begin(share, units, shares);
   s.u1 = md_share_begin(share + 1, units, shares);
   return s;
@@ -276,6 +292,110 @@ __device__ __forceinline__ MdSegments md_segments(const MdPlan& p, int claim, in
 __host__ __device__ inline int moe_decode_smem_bytes(int nt, int stages, int experts_max, int rows) {
   return 1024 + stages * (kMdStageW + nt * 128) + (2 * stages + 4 + 2 * kMdQueue) * 8 +
          (kMdQueue + 4) * 4 + (2 * experts_max + 1 + rows) * 4 + 16;
+}
+
+// CPL neighbouring fp32 columns of one lane.
+template <int CPL>
+struct MdCols {
+  float f[CPL];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) f[i] = 0.f;
+  }
+  __device__ __forceinline__ void load(const float* p) {  // past L1: other SMs wrote it
+    if constexpr (CPL == 2) {
+      const float2 a = __ldcg(reinterpret_cast<const float2*>(p));
+      f[0] = a.x, f[1] = a.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < CPL; i += 4) {
+        const float4 a = __ldcg(reinterpret_cast<const float4*>(p + i));
+        f[i] = a.x, f[i + 1] = a.y, f[i + 2] = a.z, f[i + 3] = a.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void add(const MdCols& o) {
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) f[i] += o.f[i];
+  }
+  __device__ __forceinline__ void fma(float g, const MdCols& o) {
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) f[i] = fmaf(g, o.f[i], f[i]);
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (CPL == 2) {
+      *reinterpret_cast<uint32_t*>(p) = Pack2<T>::pack(f[0], f[1]);
+    } else {
+      static_assert(CPL == 8, "16-byte stores");
+      *reinterpret_cast<uint4*>(p) =
+          make_uint4(Pack2<T>::pack(f[0], f[1]), Pack2<T>::pack(f[2], f[3]),
+                     Pack2<T>::pack(f[4], f[5]), Pack2<T>::pack(f[6], f[7]));
+    }
+  }
+};
+
+// Items first, first + stride, ... of phase 3: the gate-weighted sum of one
+// token's rows of y over 32 CPL columns, each row completed by the partials of
+// the shares that begin inside its tile.  All rows are loaded before the first
+// is used; the sum runs in slot order.
+template <typename T, int CPL>
+__device__ __forceinline__ void md_combine(const MoeDecodeArgs& args, const MdPlan& plan, int first,
+                                           int stride, int lane) {
+  const int K = args.k, topk = args.topk;
+  const int blocks = (K + 32 * CPL - 1) / (32 * CPL);
+  const size_t slot_floats = static_cast<size_t>(args.tokens) * 256;
+  using Vec = MdCols<CPL>;
+  for (int it = first; it < args.tokens * blocks; it += stride) {
+    const int t = it / blocks, col = (it - t * blocks) * 32 * CPL + lane * CPL;
+    const int nb = (it - t * blocks) * 32 * CPL / 256;
+    // Lane j: row, gate and split shares of the token's j-th expert.
+    int row = 0, base = 0, g0 = 0, g1 = 0;
+    float gate = 0.f;
+    if (lane < topk) {
+      const int as = t * topk + lane;
+      row = args.row_of[as];
+      gate = args.gates[as];
+      const int a = args.act_of[as];
+      base = row - plan.act_off[a];
+      const int u = (nb * plan.active + a) * plan.steps2;
+      g0 = md_share_of(u, plan.units2, plan.shares2) + 1;
+      g1 = md_share_of(u + plan.steps2 - 1, plan.units2, plan.shares2);
+    }
+    const bool in = col < K;
+    const int c = col & 255;
+    Vec v[kMdMaxTopk];
+#pragma unroll
+    for (int j = 0; j < kMdMaxTopk; ++j) {
+      const int r = __shfl_sync(0xffffffffu, row, j);
+      v[j].zero();
+      if (j < topk && in) v[j].load(args.y + static_cast<size_t>(r) * K + col);
+    }
+#pragma unroll
+    for (int j = 0; j < kMdMaxTopk; ++j) {
+      if (j >= topk) break;
+      const int b = __shfl_sync(0xffffffffu, base, j);
+      const int s0 = __shfl_sync(0xffffffffu, g0, j), s1 = __shfl_sync(0xffffffffu, g1, j);
+      for (int s = s0; s <= s1; s += 4) {
+        Vec w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i].zero();
+          if (s + i <= s1) w[i].load(args.part + 2 * (s + i) * slot_floats + b * 256 + c);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[j].add(w[i]);
+      }
+    }
+    Vec sum;
+    sum.zero();
+#pragma unroll
+    for (int j = 0; j < kMdMaxTopk; ++j) {
+      const float g = __shfl_sync(0xffffffffu, gate, j);
+      if (j < topk) sum.fma(g, v[j]);
+    }
+    if (in) sum.template store<T>(static_cast<T*>(args.out) + static_cast<size_t>(t) * K + col);
+  }
 }
 
 template <typename T>
@@ -301,13 +421,14 @@ __global__ void __launch_bounds__(kMdThreads, 1)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(qempty + kMdQueue) + kMdQueue;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   int* s_active = reinterpret_cast<int*>(tmem_holder + 2);
+  int* s_claim = s_active + 1;
   int* s_act_e = reinterpret_cast<int*>(tmem_holder + 4);
   const int A = args.tokens * args.topk;
   const int emax = min(args.experts, A);
   int* s_act_off = s_act_e + emax;
   int* s_row_token = s_act_off + emax + 1;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   uint32_t tmem_cols = 32;
   while (tmem_cols < 4u * nt) tmem_cols *= 2;
   if (threadIdx.x == 0) {
@@ -336,8 +457,7 @@ __global__ void __launch_bounds__(kMdThreads, 1)
   }
   pdl_allow_next();
   pdl_wait();
-  int first_claim = 0;
-  if (threadIdx.x == 0) first_claim = static_cast<int>(atomicAdd(args.header + kMdClaim, 1u));
+  if (threadIdx.x == 0) *s_claim = static_cast<int>(atomicAdd(args.header + kMdClaim, 1u));
   if (threadIdx.x == 32) *s_active = static_cast<int>(args.header[kMdActive]);
   for (int i = threadIdx.x; i < emax + 1; i += kMdThreads) {
     if (i < emax) s_act_e[i] = args.act_e[i];
@@ -360,11 +480,14 @@ __global__ void __launch_bounds__(kMdThreads, 1)
   plan.act_off = s_act_off;
   plan.row_token = s_row_token;
   const int shares = args.shares;
+  plan.shares1 = max(1, min(shares, plan.units1 / kMdMinSteps));
+  plan.shares2 = max(1, min(shares, plan.units2 / kMdMinSteps));
+  plan.claims = plan.shares1 + plan.shares2 + shares;
 
   if (warp == 0) {
     // ------------------------------------------------------- weights, claims
-    if (lane == 0) {
-      int stage = 0, claim = first_claim;
+    if (elect_one()) {
+      int stage = 0, claim = *s_claim;
       uint32_t phase = 0;
       bool ok = true;
       for (int n = 0; ok; ++n) {
@@ -372,10 +495,11 @@ __global__ void __launch_bounds__(kMdThreads, 1)
         if (!mbar_wait(&qempty[slot], ((n / kMdQueue) & 1) ^ 1, abort_flag, 31)) break;
         queue[slot] = claim;
         mbar_arrive(&qfull[slot]);
-        if (claim >= 3 * shares) break;
-        if (claim < 2 * shares) {
-          int ph;
-          MdSegments sg = md_segments(plan, claim, shares, &ph);
+        if (claim >= plan.claims) break;
+        int share;
+        const int ph = md_phase(plan, claim, &share);
+        if (ph < 2) {
+          MdSegments sg = md_segments(plan, ph, share);
           while (ok && sg.next()) {
             const int a = ph == 0 ? sg.tile / plan.tiles1 : sg.tile % plan.active;
             const int nb = ph == 0 ? sg.tile % plan.tiles1 : sg.tile / plan.active;
@@ -402,14 +526,14 @@ __global__ void __launch_bounds__(kMdThreads, 1)
           }
         }
         // A phase-3 share loads nothing here: claim the next when this one is done.
-        if (claim >= 2 * shares)
-          ok = mbar_wait(&qempty[slot], (n / kMdQueue) & 1, abort_flag, 42);
+        if (ph == 2)
+          ok = ok && mbar_wait(&qempty[slot], (n / kMdQueue) & 1, abort_flag, 42);
         if (ok) claim = static_cast<int>(atomicAdd(args.header + kMdClaim, 1u));
       }
     }
   } else if (warp == 2) {
     // ------------------------------------------------------- token operand
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true, ready = false;
@@ -418,12 +542,11 @@ __global__ void __launch_bounds__(kMdThreads, 1)
         if (!mbar_wait(&qfull[slot], (n / kMdQueue) & 1, abort_flag, 33)) break;
         const int claim = queue[slot];
         mbar_arrive(&qempty[slot]);
-        if (claim >= 2 * shares) {
-          if (claim >= 3 * shares) break;
-          continue;
-        }
-        int ph;
-        MdSegments sg = md_segments(plan, claim, shares, &ph);
+        if (claim >= plan.claims) break;
+        int share;
+        const int ph = md_phase(plan, claim, &share);
+        if (ph == 2) continue;
+        MdSegments sg = md_segments(plan, ph, share);
         while (ok && sg.next()) {
           if (ph == 1 && !ready) {
             // Every warp of phase 1 has stored its h (generic stores, read
@@ -460,7 +583,7 @@ __global__ void __launch_bounds__(kMdThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0, i = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -469,12 +592,11 @@ __global__ void __launch_bounds__(kMdThreads, 1)
         if (!mbar_wait(&qfull[slot], (n / kMdQueue) & 1, abort_flag, 36)) break;
         const int claim = queue[slot];
         mbar_arrive(&qempty[slot]);
-        if (claim >= 2 * shares) {
-          if (claim >= 3 * shares) break;
-          continue;
-        }
-        int ph;
-        MdSegments sg = md_segments(plan, claim, shares, &ph);
+        if (claim >= plan.claims) break;
+        int share;
+        const int ph = md_phase(plan, claim, &share);
+        if (ph == 2) continue;
+        MdSegments sg = md_segments(plan, ph, share);
         for (; ok && sg.next(); ++i) {
           int cols = nt;
           if (ph == 1) {
@@ -528,61 +650,26 @@ __global__ void __launch_bounds__(kMdThreads, 1)
       if (!__all_sync(0xffffffffu, ok)) break;
       const int claim = queue[qslot];
       __syncwarp();
-      if (claim >= 3 * shares) break;
-      if (claim >= 2 * shares) {
-        // --------------------------------------------- phase 3
+      if (claim >= plan.claims) break;
+      int share;
+      const int ph = md_phase(plan, claim, &share);
+      if (ph == 2) {
         ok = lane != 0 || md_wait_counter(args.header + kMdDone2,
                                           4u * static_cast<uint32_t>(plan.units2), abort_flag, 40);
         if (!__all_sync(0xffffffffu, ok)) break;
         __threadfence();
-        const int items = args.tokens * plan.tiles2;
-        const int share = claim - 2 * shares;
-        const int it1 = md_share_begin(share + 1, items, shares);
-        for (int it = md_share_begin(share, items, shares); it < it1; ++it) {
-          const int t = it / plan.tiles2, nb = it - t * plan.tiles2;
-          // Lane j: row, gate and split shares of the token's j-th expert.
-          int row = 0, base = 0, g0 = 0, g1 = 0;
-          float gate = 0.f;
-          if (lane < args.topk) {
-            const int as = t * args.topk + lane;
-            row = args.row_of[as];
-            gate = args.gates[as];
-            const int a = args.act_of[as];
-            base = row - plan.act_off[a];
-            const int u = (nb * plan.active + a) * plan.steps2;
-            g0 = md_share_of(u, plan.units2, shares) + 1;
-            g1 = md_share_of(u + plan.steps2 - 1, plan.units2, shares);
-          }
-          const int c = q * 64 + lane * 2;  // two of the block's 256 columns
-          const int col = nb * 256 + c;
-          const bool in = col < K;
-          float2 sum = make_float2(0.f, 0.f);
-          for (int j = 0; j < args.topk; ++j) {
-            const int r = __shfl_sync(0xffffffffu, row, j), b = __shfl_sync(0xffffffffu, base, j);
-            const int s0 = __shfl_sync(0xffffffffu, g0, j), s1 = __shfl_sync(0xffffffffu, g1, j);
-            const float g = __shfl_sync(0xffffffffu, gate, j);
-            float2 v = make_float2(0.f, 0.f);
-            if (in) v = __ldcg(reinterpret_cast<const float2*>(args.y + static_cast<size_t>(r) * K + col));
-            for (int s = s0; s <= s1; ++s) {
-              const float2 w = __ldcg(reinterpret_cast<const float2*>(
-                  args.part + 2 * s * slot_floats + b * 256 + c));
-              v.x += w.x;
-              v.y += w.y;
-            }
-            sum.x = fmaf(g, v.x, sum.x);
-            sum.y = fmaf(g, v.y, sum.y);
-          }
-          if (in)
-            *reinterpret_cast<uint32_t*>(static_cast<T*>(args.out) + static_cast<size_t>(t) * K + col) =
-                Pack2<T>::pack(sum.x, sum.y);
-        }
+        // One warp per item of one token and 32 CPL columns; eight columns a
+        // lane where that keeps every warp of the grid at work, two where not.
+        const int blocks = (K + 255) / 256;
+        if (args.tokens * blocks >= 4 * shares)
+          md_combine<T, 8>(args, plan, 4 * share + q, 4 * shares, lane);
+        else
+          md_combine<T, 2>(args, plan, 4 * share + q, 4 * shares, lane);
         if (lane == 0) mbar_arrive(&qempty[qslot]);
         continue;
       }
       if (lane == 0) mbar_arrive(&qempty[qslot]);
-      int ph;
-      MdSegments sg = md_segments(plan, claim, shares, &ph);
-      const int share = claim - ph * shares;
+      MdSegments sg = md_segments(plan, ph, share);
       bool stop = false;
       for (; sg.next(); ++i) {
         const int acc = i & 1;
@@ -631,8 +718,8 @@ __global__ void __launch_bounds__(kMdThreads, 1)
           bool done = whole;
           if (!whole) {
             const int u = sg.tile * plan.steps1;
-            const int s0 = md_share_of(u, plan.units1, shares);
-            const int s1 = md_share_of(u + plan.steps1 - 1, plan.units1, shares);
+            const int s0 = md_share_of(u, plan.units1, plan.shares1);
+            const int s1 = md_share_of(u + plan.steps1 - 1, plan.units1, plan.shares1);
             uint32_t seen = 0;
             __threadfence();
             __syncwarp();
@@ -643,17 +730,37 @@ __global__ void __launch_bounds__(kMdThreads, 1)
             if (seen == static_cast<uint32_t>(plan.steps1)) {
               done = true;
               __threadfence();
-              // Share s0 starts at or before the tile: slot 2 s0 + 1; the others 2 s.
-              for (int r = 0; r < m; ++r) {
-                float g = 0.f, uu = 0.f;
-                for (int s = s0; s <= s1; ++s) {
-                  const float* p = args.part + (2 * s + (s == s0)) * slot_floats + r * 256 + lcol;
-                  g += __ldcg(p);
-                  uu += __ldcg(p + 128);
+              // Share s0 starts at or before the tile: slot 2 s0 + 1; the others
+              // 2 s.  Eight rows of two shares in flight at a time.
+              for (int r0 = 0; r0 < m; r0 += 8) {
+                float g[8] = {}, uu[8] = {};
+                for (int s = s0; s <= s1; s += 2) {
+                  const float* p0 = args.part + (2 * s + (s == s0)) * slot_floats + lcol;
+                  const float* p1 = args.part + 2 * min(s + 1, s1) * slot_floats + lcol;
+                  float v[8][4];
+#pragma unroll
+                  for (int r = 0; r < 8; ++r) {
+                    const int at = min(r0 + r, m - 1) * 256;
+                    v[r][0] = __ldcg(p0 + at);
+                    v[r][1] = __ldcg(p0 + at + 128);
+                    v[r][2] = __ldcg(p1 + at);
+                    v[r][3] = __ldcg(p1 + at + 128);
+                  }
+#pragma unroll
+                  for (int r = 0; r < 8; ++r) {
+                    g[r] += v[r][0];
+                    uu[r] += v[r][1];
+                    if (s < s1) {
+                      g[r] += v[r][2];
+                      uu[r] += v[r][3];
+                    }
+                  }
                 }
-                if (col < I)
-                  h[static_cast<size_t>(row0 + r) * I + col] =
-                      Pack2<T>::from_float(g / (1.f + expf(-g)) * uu);
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                  if (r0 + r < m && col < I)
+                    h[static_cast<size_t>(row0 + r0 + r) * I + col] =
+                        Pack2<T>::from_float(g[r] / (1.f + expf(-g[r])) * uu[r]);
               }
             }
           }
