@@ -86,6 +86,8 @@ SIGNATURES = {
     "bokt_rmsnorm_row_scale": (_I32, [_VP, _VP, _I32, _I32, _F32, _I32, _VP]),
     "bokt_gemm_row_scaled": (_I32, [_VP, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _PP, _VP]),
     "bokt_rmsnorm_gemm": (_I32, [_VP, _VP, _VP, _VP, _I32, _I32, _I32, _F32, _I32, _PP, _VP]),
+    "bokt_lora_gemm_workspace_bytes": (_I64, [_I32] * 5),
+    "bokt_lora_gemm": (_I32, [_VP] * 8 + [_I32] * 6 + [_VP, _I64, _VP]),
     "bokt_qk_norm_rope": (
         _I32, [_VP] * 5 + [_I32, _VP, _I32, _VP, _VP] + [_I32] * 5 + [_VP, _I32, _F32, _I32, _VP]),
     "bokt_qk_norm_rope_workspace_bytes": (_I64, [_I32]),

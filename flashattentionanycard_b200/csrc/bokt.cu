@@ -16,6 +16,7 @@
 #include "gemm_edge.cuh"
 #include "gemm_tc.cuh"
 #include "gemm_tc2.cuh"
+#include "lora_gemm.cuh"
 #include "moe_decode.cuh"
 #include "moe_route.cuh"
 #include "norm_gemm.cuh"
@@ -1835,6 +1836,213 @@ int bokt_moe_decode(const void* x, const void* logits, int logits_dtype, const v
   void* kargs[] = {&mg, &md, &mx, &mh, &a};
   cudaError_t e = launch_ptr(fn, dim3(unsigned(a.shares)), dim3(bokt::kMdThreads), smem, s, kargs);
   if (e != cudaSuccess) return cuda_fail(e, "moe_decode launch");
+  return BOKT_OK;
+}
+
+}  // extern "C"
+
+// ----------------------------------------------------------------- projection with adapters
+namespace {
+
+// Rows up to which the weight-streaming kernel is used.
+constexpr int kLoraStreamRows = 256;
+
+struct LoraPlan {
+  bool stream;
+  int tile_rows, tiles, smax, parts, cluster, shrink_cluster, shrink_mt, stages;
+  int64_t count, list, h, total;
+};
+
+int lora_plan(int M, int N, int K, int slots, int rank, const DeviceInfo& dev, LoraPlan* p) {
+  if (M < 0 || N <= 0 || K <= 0 || slots <= 0)
+    return fail(BOKT_ERR_INVALID, "need M >= 0 and positive N, K and slots");
+  if (rank != 16 && rank != 32 && rank != 64 && rank != 128)
+    return fail(BOKT_ERR_INVALID, "padded rank must be 16, 32, 64 or 128 (got %d)", rank);
+  if (slots > bokt::kLoraMaxSlots)
+    return fail(BOKT_ERR_UNSUPPORTED, "at most %d slots (got %d)", bokt::kLoraMaxSlots, slots);
+  if (K % 8 != 0 || N % 8 != 0)
+    return fail(BOKT_ERR_UNSUPPORTED, "K and N must be multiples of 8 (got %d, %d)", K, N);
+  *p = {};
+  p->stream = M <= kLoraStreamRows;
+  if (p->stream) {
+    const int chunks = (M + 127) / 128;
+    p->tile_rows = chunks ? ((M + chunks - 1) / chunks + 15) / 16 * 16 : 16;
+    p->tiles = chunks;
+    // Split K over a cluster while that fills SMs and leaves each CTA a k-step.
+    const long long ctas = (long long)chunks * ((N + 127) / 128);
+    const int ksteps = (K + 127) / 128;
+    p->cluster = 1;
+    while (p->cluster < 8 && ctas * p->cluster * 2 <= dev.sm_count && ksteps >= p->cluster * 2)
+      p->cluster *= 2;
+    p->stages = 8;
+    while (p->stages > 2 && bokt::lora_stream_smem_bytes(p->tile_rows, p->stages) > dev.smem_optin)
+      --p->stages;
+  } else {
+    p->tile_rows = bokt::kLoraPairRows;
+    p->tiles = (M + bokt::kLoraPairRows - 1) / bokt::kLoraPairRows;
+    p->cluster = 2;
+    p->stages = 6;
+  }
+  // The shrink: 32 tokens per cluster halve the reads of A, where enough
+  // clusters remain; few tokens split K over up to eight CTAs.
+  p->shrink_mt = M >= 2048 ? 2 : 1;
+  const long long clusters = (M + 16 * p->shrink_mt - 1) / (16 * p->shrink_mt);
+  p->shrink_cluster = 1;
+  while (p->shrink_cluster < 8 && clusters * p->shrink_cluster * 2 <= dev.sm_count &&
+         K >= p->shrink_cluster * 2 * 8 * 32)
+    p->shrink_cluster *= 2;
+  p->smax = slots < p->tile_rows ? slots : p->tile_rows;
+  p->parts = rank > 64 ? 2 : 1;
+  const int64_t entries = (int64_t)p->tiles * p->smax;
+  if (entries * p->tile_rows > 0x7fffffffLL)
+    return fail(BOKT_ERR_UNSUPPORTED, "too many rows and adapters (M=%d, slots=%d)", M, slots);
+  auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
+  p->count = 0;
+  p->list = up((int64_t)p->tiles * 4);
+  p->h = p->list + up(entries * 4);
+  p->total = p->h + up(entries * p->tile_rows * 64 * p->parts * 2);
+  if (p->total < 256) p->total = 256;
+  return BOKT_OK;
+}
+
+cudaError_t launch_cluster(const void* fn, int grid, int threads, int smem, int cluster,
+                           cudaStream_t s, void** kargs) {
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t lc = launch_config(dim3(unsigned(grid)), dim3(unsigned(threads)), smem, s, attr);
+  attr[lc.numAttrs].id = cudaLaunchAttributeClusterDimension;
+  attr[lc.numAttrs].val.clusterDim.x = unsigned(cluster);
+  attr[lc.numAttrs].val.clusterDim.y = 1;
+  attr[lc.numAttrs].val.clusterDim.z = 1;
+  lc.numAttrs += 1;
+  return cudaLaunchKernelExC(&lc, fn, kargs);
+}
+
+template <typename T, int MT>
+const void* lora_shrink_ptr(int rank) {
+  if (rank == 16) return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, MT, 2>);
+  if (rank == 32) return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, MT, 4>);
+  return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, MT, 8>);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t bokt_lora_gemm_workspace_bytes(int M, int N, int K, int slots, int rank) {
+  g_err[0] = 0;
+  DeviceInfo dev;
+  LoraPlan p;
+  if (device_info(&dev) || lora_plan(M, N, K, slots, rank, dev, &p)) return -1;
+  return p.total;
+}
+
+int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void* lora_b,
+                   const float* scales, const int32_t* ranks, const int32_t* ids, void* out, int M,
+                   int N, int K, int slots, int rank, int dtype, void* workspace,
+                   int64_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  if (dtype != BOKT_FP16 && dtype != BOKT_BF16) return fail(BOKT_ERR_INVALID, "dtype %d", dtype);
+  DeviceInfo dev = {};
+  LoraPlan p;
+  int rc = lora_plan(M, N, K, slots, rank, dev, &p);  // sizes, before any device call
+  if (rc) return rc;
+  if (M == 0) return BOKT_OK;
+  if (!x || !W || !lora_a || !lora_b || !scales || !ranks || !ids || !out || !workspace)
+    return fail(BOKT_ERR_INVALID, "null pointer");
+  if (!aligned16(x) || !aligned16(W) || !aligned16(lora_a) || !aligned16(lora_b) || !aligned16(out))
+    return fail(BOKT_ERR_UNSUPPORTED, "x, W, the adapters and out must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return fail(BOKT_ERR_INVALID, "workspace must be 256-byte aligned");
+  rc = device_info(&dev);
+  if (rc) return rc;
+  rc = lora_plan(M, N, K, slots, rank, dev, &p);
+  if (rc) return rc;
+  if (workspace_bytes < p.total)
+    return fail(BOKT_ERR_INVALID, "workspace too small: %lld bytes, need %lld",
+                (long long)workspace_bytes, (long long)p.total);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  bokt::LoraArgs a = {};
+  a.M = M, a.N = N, a.K = K, a.slots = slots, a.rank = rank;
+  a.tile_rows = p.tile_rows, a.smax = p.smax, a.parts = p.parts;
+  a.ids = ids, a.ranks = ranks, a.scales = scales;
+  a.count = reinterpret_cast<int32_t*>(ws + p.count);
+  a.list = reinterpret_cast<int32_t*>(ws + p.list);
+  a.h = ws + p.h;
+  a.out = out;
+  a.chunks = p.tiles;
+  const bool fp16 = dtype == BOKT_FP16;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+
+  CUtensorMap mx, mw, mh, mb;
+  const uint32_t rs = uint32_t(rank < 64 ? rank : 64);
+  {
+    const uint64_t d[2] = {uint64_t(K), uint64_t(M)};
+    const uint64_t st[1] = {uint64_t(K) * 2};
+    const uint32_t b[2] = {64, p.stream ? uint32_t(p.tile_rows) : 128u};
+    if ((rc = encode_map(&mx, x, 2, d, st, b, fp16))) return rc;
+  }
+  {
+    const uint64_t d[2] = {uint64_t(N), uint64_t(K)};
+    const uint64_t st[1] = {uint64_t(N) * 2};
+    const uint32_t b[2] = {64, 64};
+    if ((rc = encode_map(&mw, W, 2, d, st, b, fp16))) return rc;
+  }
+  {
+    const uint64_t width = uint64_t(64) * p.parts;
+    const uint64_t d[2] = {width, uint64_t(p.tiles) * p.smax * p.tile_rows};
+    const uint64_t st[1] = {width * 2};
+    const uint32_t b[2] = {64, p.stream ? uint32_t(p.tile_rows) : 128u};
+    if ((rc = encode_map(&mh, a.h, 2, d, st, b, fp16))) return rc;
+  }
+  {
+    const uint64_t d[3] = {uint64_t(N), uint64_t(rank), uint64_t(slots)};
+    const uint64_t st[2] = {uint64_t(N) * 2, uint64_t(N) * 2 * rank};
+    const uint32_t b[3] = {64, rs, 1};
+    if ((rc = encode_map(&mb, lora_b, 3, d, st, b, fp16))) return rc;
+  }
+  {
+    const bool bf = dtype == BOKT_BF16;
+    const void* fn = p.shrink_mt == 2 ? (bf ? lora_shrink_ptr<__nv_bfloat16, 2>(rank)
+                                            : lora_shrink_ptr<__half, 2>(rank))
+                                      : (bf ? lora_shrink_ptr<__nv_bfloat16, 1>(rank)
+                                            : lora_shrink_ptr<__half, 1>(rank));
+    const int smem = p.shrink_mt == 2 ? bokt::lora_shrink_smem_bytes<2>() : bokt::lora_shrink_smem_bytes<1>();
+    if ((rc = ensure_smem(fn, smem))) return rc;
+    const int clusters = (M + 16 * p.shrink_mt - 1) / (16 * p.shrink_mt);
+    a.cluster = p.shrink_cluster;
+    void* kargs[] = {&x, &lora_a, &a};
+    cudaError_t e = launch_cluster(fn, clusters * a.cluster, bokt::kLoraThreads, smem, a.cluster, s, kargs);
+    if (e != cudaSuccess) return cuda_fail(e, "lora_shrink launch");
+  }
+  a.cluster = p.cluster;
+  a.stages = p.stages;
+  cudaError_t e;
+  if (p.stream) {
+    a.idesc = bokt::make_idesc_f16_swapped(uint32_t(dtype), uint32_t(p.tile_rows));
+    const void* fn = fp16 ? reinterpret_cast<const void*>(&bokt::lora_stream_kernel<__half>)
+                          : reinterpret_cast<const void*>(&bokt::lora_stream_kernel<__nv_bfloat16>);
+    int smem = bokt::lora_stream_smem_bytes(p.tile_rows, p.stages);
+    if (smem < dev.smem_optin / 2 + 1024) smem = dev.smem_optin / 2 + 1024;  // one CTA per SM
+    if ((rc = ensure_smem(fn, smem))) return rc;
+    const long long grid = (long long)p.tiles * ((N + 127) / 128) * p.cluster;
+    if (grid > 0x7fffffffLL) return fail(BOKT_ERR_UNSUPPORTED, "too many tiles");
+    void* kargs[] = {&mw, &mx, &mb, &mh, &a};
+    e = launch_cluster(fn, int(grid), bokt::kLoraThreads, smem, p.cluster, s, kargs);
+  } else {
+    a.idesc = bokt::make_idesc_f16(uint32_t(dtype), 256, 256);
+    a.group_m = 8;
+    const void* fn = fp16 ? reinterpret_cast<const void*>(&bokt::lora_tc2_kernel<__half>)
+                          : reinterpret_cast<const void*>(&bokt::lora_tc2_kernel<__nv_bfloat16>);
+    const int smem = bokt::lora_tc2_smem_bytes(p.stages);
+    if (smem > dev.smem_optin) return fail(BOKT_ERR_UNSUPPORTED, "needs %d bytes of shared memory", smem);
+    if ((rc = ensure_smem(fn, smem))) return rc;
+    const long long tiles = (long long)p.tiles * ((N + 255) / 256);
+    if (tiles > 0x7fffffffLL) return fail(BOKT_ERR_UNSUPPORTED, "too many tiles");
+    const int pairs = int(tiles < dev.sm_count / 2 ? tiles : dev.sm_count / 2);
+    void* kargs[] = {&mx, &mw, &mh, &mb, &a};
+    e = launch_cluster(fn, 2 * pairs, bokt::kGemmThreads, smem, 2, s, kargs);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, "lora product launch");
   return BOKT_OK;
 }
 

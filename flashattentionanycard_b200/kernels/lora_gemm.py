@@ -1,0 +1,137 @@
+"""A shared projection with the low-rank adapters of many requests at once (sm_100a).
+
+The dense GEMM of the reference's ``bo_kernel_tuner/kernels/gemm.py:7-40`` with
+one adapter per row beside it (the reference has none):
+
+    out[t] = x[t] @ w + scale_a * (x[t] @ A_a.T) @ B_a     a = ids[t], -1: none
+
+An ``AdapterBank`` keeps the adapters of a projection in slots on the device, as
+a serving program loads them; ``launch`` runs a batch in which every row names
+its slot, in two kernels: the rows' low-rank vectors, then the projection, whose
+K loop goes on over the adapters that the row tile uses.  Up to 256 rows the
+second kernel streams ``w`` against the tokens (decode); above, it is the
+CTA-pair GEMM (prefill).
+"""
+
+import math
+
+from flashattentionanycard_b200 import _native
+
+MAX_SLOTS, RANKS = 1024, (16, 32, 64, 128)
+
+
+class AdapterBank:
+    """Adapters of one [K, N] projection in ``slots`` device slots, ranks up to ``max_rank``.
+
+    ``load`` copies an adapter in (on the current stream) and refuses values
+    that are not finite: rows of other adapters meet them as zero factors."""
+
+    def __init__(self, slots, k, n, max_rank, dtype, device):
+        import torch
+
+        self.slots, self.k, self.n = int(slots), int(k), int(n)
+        if not 1 <= self.slots <= MAX_SLOTS:
+            raise ValueError(f"slots must be in [1, {MAX_SLOTS}], got {slots}")
+        if self.k < 8 or self.n < 8 or self.k % 8 or self.n % 8:
+            raise ValueError(f"K and N must be positive multiples of 8 (got {k} and {n})")
+        if not 1 <= int(max_rank) <= RANKS[-1]:
+            raise ValueError(f"max_rank must be in [1, {RANKS[-1]}], got {max_rank}")
+        _native.dtype_code(dtype)
+        self.rank = next(r for r in RANKS if r >= int(max_rank))
+        self.max_rank = int(max_rank)
+        self.a = torch.zeros(self.slots, self.rank, self.k, dtype=dtype, device=device)
+        self.b = torch.zeros(self.slots, self.rank, self.n, dtype=dtype, device=device)
+        self.scales = torch.zeros(self.slots, dtype=torch.float32, device=device)
+        self.ranks = torch.zeros(self.slots, dtype=torch.int32, device=device)
+        self.dtype, self.device = dtype, self.a.device
+
+    def _slot(self, slot):
+        if not 0 <= int(slot) < self.slots:
+            raise ValueError(f"slot must be in [0, {self.slots}), got {slot}")
+        return int(slot)
+
+    def load(self, slot, a, b, scale=1.0):
+        """Put the adapter a [r, K], b [r, N] with its scale into ``slot``."""
+        import torch
+
+        slot = self._slot(slot)
+        r = a.shape[0]
+        if a.dim() != 2 or b.dim() != 2 or not 1 <= r <= self.max_rank \
+                or a.shape != (r, self.k) or b.shape != (r, self.n):
+            raise ValueError(f"shape mismatch: a {tuple(a.shape)}, b {tuple(b.shape)}; expected [r, {self.k}] "
+                             f"and [r, {self.n}] with r in [1, {self.max_rank}]")
+        if a.dtype != self.dtype or b.dtype != self.dtype:
+            raise ValueError(f"the adapter must have the bank's dtype {self.dtype}")
+        scale = float(scale)
+        if not math.isfinite(scale) or not math.isfinite(torch.tensor(scale, dtype=torch.float32).item()):
+            raise ValueError("scale must be a finite fp32 value")
+        if not (torch.isfinite(a).all() and torch.isfinite(b).all()):
+            raise ValueError("the adapter holds values that are not finite")
+        self.unload(slot)
+        self.a[slot, :r].copy_(a)
+        self.b[slot, :r].copy_(b)
+        self.scales[slot] = scale
+        self.ranks[slot] = r
+
+    def unload(self, slot):
+        slot = self._slot(slot)
+        self.ranks[slot] = 0
+        self.scales[slot] = 0
+        self.a[slot].zero_()
+        self.b[slot].zero_()
+
+
+def workspace_bytes(m, bank):
+    """Device scratch of one call with m rows on the current device."""
+    lib = _native.load()
+    n = int(lib.bokt_lora_gemm_workspace_bytes(int(m), bank.n, bank.k, bank.slots, bank.rank))
+    if n < 0:
+        raise RuntimeError(f"bokt_lora_gemm_workspace_bytes: {lib.bokt_last_error().decode()}")
+    return n
+
+
+def launch(x, w, bank, ids, out, workspace=None):
+    """out[T, N] = x[T, K] @ w[K, N] plus every row's adapter; ids int32 [T], -1 for none.
+
+    An id outside [-1, slots) or of an empty slot sets the device status word
+    (``_native.device_status``), and its row gets the projection alone.
+    ``workspace``: a uint8 tensor of ``workspace_bytes`` (calls that may overlap
+    on the GPU need one each); by default the call takes a fresh one from
+    torch's allocator."""
+    import torch
+
+    m, k = x.shape
+    n = w.shape[1]
+    if w.shape[0] != k or out.shape != (m, n):
+        raise ValueError(f"shape mismatch: x {tuple(x.shape)}, w {tuple(w.shape)}, out {tuple(out.shape)}")
+    if (k, n) != (bank.k, bank.n):
+        raise ValueError(f"the bank's adapters are for a [{bank.k}, {bank.n}] projection, not [{k}, {n}]")
+    if ids.dtype != torch.int32 or ids.shape != (m,) or not ids.is_contiguous():
+        raise ValueError(f"ids must be a contiguous int32 tensor of {m} elements")
+    if not (x.dtype == w.dtype == out.dtype == bank.dtype):
+        raise ValueError("x, w, out and the bank must share one dtype")
+    if not (x.is_contiguous() and w.is_contiguous() and out.is_contiguous()):
+        raise ValueError("x, w and out must be contiguous row-major tensors")
+    device = x.device
+    if not (x.is_cuda and w.device == device and out.device == device and ids.device == device
+            and bank.device == device):
+        raise ValueError("all tensors and the bank must be on one CUDA device")
+    lib = _native.load()
+    with _native.on_device(device):
+        need = lib.bokt_lora_gemm_workspace_bytes(m, n, k, bank.slots, bank.rank)
+        if need < 0:
+            raise RuntimeError(f"bokt_lora_gemm: {lib.bokt_last_error().decode()}")
+        if workspace is None:
+            workspace = torch.empty(need, device=device, dtype=torch.uint8)
+        elif workspace.device != device or not workspace.is_contiguous() \
+                or workspace.numel() * workspace.element_size() < need:
+            raise ValueError(f"workspace must be a contiguous tensor of {need} bytes on {device}")
+        _native.check(
+            lib.bokt_lora_gemm(
+                x.data_ptr(), w.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
+                bank.ranks.data_ptr(), ids.data_ptr(), out.data_ptr(), m, n, k, bank.slots, bank.rank,
+                _native.dtype_code(x.dtype), workspace.data_ptr(),
+                workspace.numel() * workspace.element_size(), _native.current_stream(device)),
+            "bokt_lora_gemm",
+        )
+    return out

@@ -208,6 +208,29 @@ int bokt_rmsnorm_gemm(const void* X, const void* B_folded, void* C, float* row_s
                       void* stream);
 
 /*
+ * A shared projection with one low-rank adapter per row (two kernels):
+ *   out[m] = x[m] W + scales[a] (x[m] A_a^T) B_a,   a = ids[m]; a = -1: x[m] W
+ * x [M, K], W [K, N], lora_a [slots, rank, K], lora_b [slots, rank, N], out
+ * [M, N] of one type; scales fp32 [slots]; ranks int32 [slots]: the adapter's
+ * own rank (rows past it are zero), 0 for an empty slot; ids int32 [M].  The
+ * adapters in use are read once per row tile and join the projection's fp32
+ * accumulator; scales[a] (x A_a^T) is rounded to the type (it is a tensor-core
+ * operand), the sum once.  lora_b must be finite: rows of other adapters
+ * multiply it by zero.  An id outside [-1, slots) or of an empty slot sets the
+ * device status word (code 6) and its row gets x W alone.  rank: 16, 32, 64 or
+ * 128; slots <= 1024; K and N multiples of 8; 16-byte aligned pointers.
+ * workspace: bokt_lora_gemm_workspace_bytes(...) bytes of device scratch,
+ * 256-byte aligned, contents free before and after; calls that overlap on the
+ * GPU need one each.  The product is that of kernels/gemm.py:7-40; adapters
+ * have no counterpart in the reference.
+ */
+int64_t bokt_lora_gemm_workspace_bytes(int M, int N, int K, int slots, int rank);
+int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void* lora_b,
+                   const float* scales, const int32_t* ranks, const int32_t* ids, void* out, int M,
+                   int N, int K, int slots, int rank, int dtype, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/*
  * RMSNorm of every query and key head and the rotary position rotation in one
  * pass.  q [tokens, heads, dim] and k [tokens, kv_heads, dim] are views with
  * element strides (last dimension contiguous), as the projection leaves them

@@ -1,0 +1,101 @@
+"""Refusals of the adapter bank and the projection with adapters (no GPU needed)."""
+
+import pytest
+import torch
+
+from flashattentionanycard_b200 import _native
+from flashattentionanycard_b200.kernels import lora_gemm
+
+BF = torch.bfloat16
+
+
+def bank(**over):
+    return lora_gemm.AdapterBank(**{**dict(slots=4, k=16, n=24, max_rank=8, dtype=BF, device="cpu"), **over})
+
+
+@pytest.mark.parametrize("over, match", [
+    (dict(slots=0), "slots"), (dict(slots=1025), "slots"), (dict(k=12), "multiples of 8"),
+    (dict(n=0), "multiples of 8"), (dict(max_rank=0), "max_rank"), (dict(max_rank=129), "max_rank"),
+    (dict(dtype=torch.float32), "dtype"),
+])
+def test_bank_refusals(over, match):
+    with pytest.raises(ValueError, match=match):
+        bank(**over)
+
+
+def test_bank_load_and_unload():
+    b = bank()
+    assert b.rank == 16
+    a1, b1 = torch.randn(8, 16).to(BF), torch.randn(8, 24).to(BF)
+    b.load(2, a1, b1, 0.5)
+    assert torch.equal(b.a[2, :8], a1) and torch.equal(b.b[2, :8], b1)
+    assert not b.a[2, 8:].any() and b.ranks.tolist() == [0, 0, 8, 0] and b.scales[2] == 0.5
+    b.load(2, a1[:3], b1[:3])  # a smaller adapter leaves nothing of the larger one
+    assert not b.a[2, 3:].any() and not b.b[2, 3:].any() and b.ranks[2] == 3
+    b.unload(2)
+    assert not b.a.any() and not b.b.any() and not b.ranks.any() and not b.scales.any()
+
+
+@pytest.mark.parametrize("args, match", [
+    ((4, (8, 16), (8, 24)), "slot"), ((-1, (8, 16), (8, 24)), "slot"),
+    ((0, (9, 16), (9, 24)), "shape mismatch"), ((0, (0, 16), (0, 24)), "shape mismatch"),
+    ((0, (8, 24), (8, 24)), "shape mismatch"), ((0, (8, 16), (7, 24)), "shape mismatch"),
+])
+def test_load_refusals(args, match):
+    slot, a, b = args
+    with pytest.raises(ValueError, match=match):
+        bank().load(slot, torch.zeros(a, dtype=BF), torch.zeros(b, dtype=BF))
+
+
+def test_load_refuses_types_and_values_that_are_not_finite():
+    b, a1, b1 = bank(), torch.zeros(4, 16, dtype=BF), torch.zeros(4, 24, dtype=BF)
+    with pytest.raises(ValueError, match="dtype"):
+        b.load(0, a1.half(), b1)
+    for scale in (float("inf"), float("nan"), 1e39):
+        with pytest.raises(ValueError, match="scale"):
+            b.load(0, a1, b1, scale)
+    for bad in (float("inf"), float("nan")):
+        x = b1.clone()
+        x[3, 7] = bad
+        with pytest.raises(ValueError, match="finite"):
+            b.load(0, a1, x)
+        x = a1.clone()
+        x[0, 0] = bad
+        with pytest.raises(ValueError, match="finite"):
+            b.load(0, x, b1)
+    assert not b.ranks.any()
+
+
+def call(t=3, **over):
+    a = {"x": torch.zeros(t, 16, dtype=BF), "w": torch.zeros(16, 24, dtype=BF), "bank": bank(),
+         "ids": torch.zeros(t, dtype=torch.int32), "out": torch.zeros(t, 24, dtype=BF)}
+    return lora_gemm.launch(**{**a, **over})
+
+
+@pytest.mark.parametrize("over, match", [
+    (dict(w=torch.zeros(24, 24, dtype=BF)), "shape mismatch"),
+    (dict(out=torch.zeros(4, 24, dtype=BF)), "shape mismatch"),
+    (dict(bank=bank(n=32)), "bank"),
+    (dict(ids=torch.zeros(4, dtype=torch.int32)), "ids"),
+    (dict(ids=torch.zeros(3, dtype=torch.int64)), "ids"),
+    (dict(ids=torch.zeros(6, dtype=torch.int32)[::2]), "ids"),
+    (dict(bank=bank(dtype=torch.float16)), "share one dtype"),
+    (dict(x=torch.zeros(16, 3, dtype=BF).t()), "contiguous"),
+    ({}, "CUDA"),
+])
+def test_launch_refusals(over, match):
+    with pytest.raises(ValueError, match=match):
+        call(**over)
+
+
+def test_c_abi_argument_errors_need_no_gpu():
+    lib = _native.load()
+
+    def rc(m=1, n=8, k=8, slots=1, rank=16, dtype=1):
+        return lib.bokt_lora_gemm(*[None] * 8, m, n, k, slots, rank, dtype, None, 0, None)
+
+    assert rc(dtype=2) == 1 and b"dtype" in lib.bokt_last_error()
+    assert rc(m=-1) == 1 and rc(n=0) == 1 and rc(slots=0) == 1 and rc(rank=24) == 1
+    assert rc(slots=1025) == 2 and rc(k=12) == 2 and rc(n=4) == 2
+    assert rc(m=0) == 0
+    assert rc() == 1 and b"null" in lib.bokt_last_error()
