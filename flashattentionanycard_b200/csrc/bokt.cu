@@ -1846,12 +1846,46 @@ namespace {
 
 // Rows up to which the weight-streaming kernel is used.
 constexpr int kLoraStreamRows = 256;
+// Shared memory left to a shrink CTA (rank 16: 9 KB of partials, 7 KB of lists).
+constexpr int kLoraShrinkSmem = 20 * 1024;
 
 struct LoraPlan {
   bool stream;
-  int tile_rows, tiles, smax, parts, cluster, shrink_cluster, shrink_mt, stages;
+  int tile_rows, tiles, smax, gmax, cluster, stages;
+  int shrink_cluster, shrink_mt, walkers;
   int64_t count, list, h, total;
 };
+
+// Clusters of `cluster` stream-kernel CTAs (one per SM) that the current device
+// holds at once: a cluster keeps to one GPC, so fewer than sm_count / cluster.
+int lora_cluster_room(const DeviceInfo& dev, int cluster) {
+  if (dev.sm_count == 0) return 0;
+  static int room[kMaxDevices][4];
+  static std::mutex mu;
+  int d = 0;
+  cudaGetDevice(&d);
+  const int at = cluster == 2 ? 0 : cluster == 4 ? 1 : 2;
+  std::lock_guard<std::mutex> lock(mu);
+  if (room[d][at] == 0) {
+    const void* fn = reinterpret_cast<const void*>(&bokt::lora_stream_kernel<__nv_bfloat16>);
+    if (ensure_smem(fn, dev.smem_optin)) return 0;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(cluster);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(unsigned(dev.sm_count / cluster * cluster));
+    lc.blockDim = dim3(bokt::kLoraThreads);
+    lc.dynamicSmemBytes = dev.smem_optin;
+    lc.attrs = attr;
+    lc.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, fn, &lc) != cudaSuccess) n = 0;
+    room[d][at] = n > 0 ? n : -1;
+  }
+  return room[d][at];
+}
 
 int lora_plan(int M, int N, int K, int slots, int rank, const DeviceInfo& dev, LoraPlan* p) {
   if (M < 0 || N <= 0 || K <= 0 || slots <= 0)
@@ -1866,16 +1900,23 @@ int lora_plan(int M, int N, int K, int slots, int rank, const DeviceInfo& dev, L
   p->stream = M <= kLoraStreamRows;
   if (p->stream) {
     const int chunks = (M + 127) / 128;
-    p->tile_rows = chunks ? ((M + chunks - 1) / chunks + 15) / 16 * 16 : 16;
     p->tiles = chunks;
-    // Split K over a cluster while that fills SMs and leaves each CTA a k-step.
+    // Split K over a cluster while that fills SMs (all clusters resident at
+    // once) and leaves each CTA a k-step.
     const long long ctas = (long long)chunks * ((N + 127) / 128);
     const int ksteps = (K + 127) / 128;
     p->cluster = 1;
-    while (p->cluster < 8 && ctas * p->cluster * 2 <= dev.sm_count && ksteps >= p->cluster * 2)
+    while (p->cluster < 8 && ctas <= lora_cluster_room(dev, p->cluster * 2) &&
+           ksteps >= p->cluster * 2)
       p->cluster *= 2;
+    // Each CTA of a cluster finishes its own quads of tokens.
+    const int unit = 4 * p->cluster > 16 ? 4 * p->cluster : 16;
+    p->tile_rows = chunks ? ((M + chunks - 1) / chunks + unit - 1) / unit * unit : 16;
+    // Leave room beside the shrink kernel's CTAs, so that the W stream starts
+    // while they run.
     p->stages = 8;
-    while (p->stages > 2 && bokt::lora_stream_smem_bytes(p->tile_rows, p->stages) > dev.smem_optin)
+    while (p->stages > 2 &&
+           bokt::lora_stream_smem_bytes(p->tile_rows, p->stages) > dev.smem_optin - kLoraShrinkSmem)
       --p->stages;
   } else {
     p->tile_rows = bokt::kLoraPairRows;
@@ -1883,24 +1924,27 @@ int lora_plan(int M, int N, int K, int slots, int rank, const DeviceInfo& dev, L
     p->cluster = 2;
     p->stages = 6;
   }
-  // The shrink: 32 tokens per cluster halve the reads of A, where enough
-  // clusters remain; few tokens split K over up to eight CTAs.
-  p->shrink_mt = M >= 2048 ? 2 : 1;
-  const long long clusters = (M + 16 * p->shrink_mt - 1) / (16 * p->shrink_mt);
-  p->shrink_cluster = 1;
-  while (p->shrink_cluster < 8 && clusters * p->shrink_cluster * 2 <= dev.sm_count &&
-         K >= p->shrink_cluster * 2 * 8 * 32)
-    p->shrink_cluster *= 2;
   p->smax = slots < p->tile_rows ? slots : p->tile_rows;
-  p->parts = rank > 64 ? 2 : 1;
-  const int64_t entries = (int64_t)p->tiles * p->smax;
-  if (entries * p->tile_rows > 0x7fffffffLL)
+  if (M < p->smax && M > 0) p->smax = M;
+  // The shrink: row tiles of many tokens walk an adapter's tokens 32 at a time
+  // over clusters of eight CTAs; few tokens split K as far as there are SMs.
+  p->shrink_mt = p->stream ? 1 : 2;
+  p->shrink_cluster = 8;
+  if (p->stream)
+    while (p->shrink_cluster > 1 && ((long long)p->tiles * p->smax * p->shrink_cluster > dev.sm_count ||
+                                     K < p->shrink_cluster * 256))
+      p->shrink_cluster /= 2;
+  const long long want = dev.sm_count / ((long long)p->shrink_cluster * (p->tiles ? p->tiles : 1));
+  p->walkers = int(want < 1 ? 1 : (want < p->smax ? want : p->smax));
+  p->gmax = (p->smax * rank + 63) / 64;
+  const int64_t entries = (int64_t)p->tiles * p->smax, groups = (int64_t)p->tiles * p->gmax;
+  if (groups * p->tile_rows > 0x7fffffffLL)
     return fail(BOKT_ERR_UNSUPPORTED, "too many rows and adapters (M=%d, slots=%d)", M, slots);
   auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
   p->count = 0;
   p->list = up((int64_t)p->tiles * 4);
   p->h = p->list + up(entries * 4);
-  p->total = p->h + up(entries * p->tile_rows * 64 * p->parts * 2);
+  p->total = p->h + up(groups * p->tile_rows * 64 * 2);
   if (p->total < 256) p->total = 256;
   return BOKT_OK;
 }
@@ -1918,9 +1962,16 @@ cudaError_t launch_cluster(const void* fn, int grid, int threads, int smem, int 
 }
 
 template <typename T, int MT>
-const void* lora_shrink_ptr(int rank) {
-  if (rank == 16) return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, MT, 2>);
-  if (rank == 32) return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, MT, 4>);
+const void* lora_shrink_ptr(int rank, int* smem) {
+  if (rank == 16) {
+    *smem = bokt::lora_shrink_smem_bytes<MT, 2>();
+    return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, MT, 2>);
+  }
+  if (rank == 32) {
+    *smem = bokt::lora_shrink_smem_bytes<MT, 4>();
+    return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, MT, 4>);
+  }
+  *smem = bokt::lora_shrink_smem_bytes<MT, 8>();
   return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, MT, 8>);
 }
 
@@ -1963,7 +2014,7 @@ int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void*
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   bokt::LoraArgs a = {};
   a.M = M, a.N = N, a.K = K, a.slots = slots, a.rank = rank;
-  a.tile_rows = p.tile_rows, a.smax = p.smax, a.parts = p.parts;
+  a.tile_rows = p.tile_rows, a.smax = p.smax, a.gmax = p.gmax;
   a.ids = ids, a.ranks = ranks, a.scales = scales;
   a.count = reinterpret_cast<int32_t*>(ws + p.count);
   a.list = reinterpret_cast<int32_t*>(ws + p.list);
@@ -1988,9 +2039,8 @@ int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void*
     if ((rc = encode_map(&mw, W, 2, d, st, b, fp16))) return rc;
   }
   {
-    const uint64_t width = uint64_t(64) * p.parts;
-    const uint64_t d[2] = {width, uint64_t(p.tiles) * p.smax * p.tile_rows};
-    const uint64_t st[1] = {width * 2};
+    const uint64_t d[2] = {64, uint64_t(p.tiles) * p.gmax * p.tile_rows};
+    const uint64_t st[1] = {128};
     const uint32_t b[2] = {64, p.stream ? uint32_t(p.tile_rows) : 128u};
     if ((rc = encode_map(&mh, a.h, 2, d, st, b, fp16))) return rc;
   }
@@ -2002,14 +2052,15 @@ int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void*
   }
   {
     const bool bf = dtype == BOKT_BF16;
-    const void* fn = p.shrink_mt == 2 ? (bf ? lora_shrink_ptr<__nv_bfloat16, 2>(rank)
-                                            : lora_shrink_ptr<__half, 2>(rank))
-                                      : (bf ? lora_shrink_ptr<__nv_bfloat16, 1>(rank)
-                                            : lora_shrink_ptr<__half, 1>(rank));
-    const int smem = p.shrink_mt == 2 ? bokt::lora_shrink_smem_bytes<2>() : bokt::lora_shrink_smem_bytes<1>();
+    int smem = 0;
+    const void* fn = p.shrink_mt == 2 ? (bf ? lora_shrink_ptr<__nv_bfloat16, 2>(rank, &smem)
+                                            : lora_shrink_ptr<__half, 2>(rank, &smem))
+                                      : (bf ? lora_shrink_ptr<__nv_bfloat16, 1>(rank, &smem)
+                                            : lora_shrink_ptr<__half, 1>(rank, &smem));
     if ((rc = ensure_smem(fn, smem))) return rc;
-    const int clusters = (M + 16 * p.shrink_mt - 1) / (16 * p.shrink_mt);
+    const int clusters = p.tiles * p.walkers;
     a.cluster = p.shrink_cluster;
+    a.walkers = p.walkers;
     void* kargs[] = {&x, &lora_a, &a};
     cudaError_t e = launch_cluster(fn, clusters * a.cluster, bokt::kLoraThreads, smem, a.cluster, s, kargs);
     if (e != cudaSuccess) return cuda_fail(e, "lora_shrink launch");

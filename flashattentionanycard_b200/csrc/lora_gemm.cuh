@@ -5,15 +5,16 @@
 // The adapters' second product joins the projection's own K loop: with
 //   H_j[t] = s_a (x[t] A_a^T) where ids[t] = a_j, else 0
 // for the adapters a_j of a row tile, the tile is x W + sum_j H_j B_{a_j}: the
-// tile's accumulator runs R more k-values per adapter in use, and nothing is
-// read back or rounded in between.  H is rounded to the element type (it is a
+// tile's accumulator runs R more k-values per adapter in use, 64 / R adapters to
+// a 64-deep step, and nothing is read back or rounded in between.  H is rounded to the element type (it is a
 // tensor-core operand).  The zeros of H_j meet B of other tokens' adapters, so
 // B must be finite; the bank refuses adapters that are not.
 //
 //   lora_shrink_kernel  H (and each row tile's list of adapters).  HBM / latency
-//       bound; 16 or 32 tokens a cluster, K split over its warps and CTAs,
-//       warp-level mma.sync on fragments loaded straight from global memory
-//       (few flops: a tcgen05 tile would idle on 16 columns).
+//       bound; a cluster per (row tile, adapter), its tokens gathered 16 or 32
+//       at a time, K split over warps and CTAs; warp-level mma.sync on fragments
+//       loaded straight from global memory (few flops: a 128-row tcgen05 tile
+//       would idle on an adapter's handful of tokens).
 //   lora_stream_kernel  few tokens (row tiles of up to 128): bound by reading W.
 //       W tiles are the 128-row operand and the tokens the narrow one; a cluster
 //       of C CTAs splits K and reduces through distributed shared memory.
@@ -43,9 +44,11 @@ struct LoraArgs {
   const float* scales;    // [slots]
   int32_t* count;         // [row tiles] adapters in use
   int32_t* list;          // [row tiles][smax]
-  void* h;                // [row tiles][smax][tile_rows][64 * parts]
+  void* h;                // [row tiles][gmax][tile_rows][64]: entry j's R columns start at
+                          // column j R of the tile's gmax x 64
   void* out;
-  int parts;              // 64-wide parts of a row of H (1 or 2)
+  int gmax;               // 64-wide groups of columns per row tile
+  int walkers;            // shrink: clusters per row tile, each walking every walkers-th entry
   int cluster;            // CTAs per cluster of the kernel at hand
   int stages, group_m, chunks;
   uint32_t idesc;
@@ -75,54 +78,64 @@ __device__ __forceinline__ void mma_16816<__half>(float (&c)[4], uint32_t a0, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+__device__ __forceinline__ void st_cluster_u32x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                                 uint32_t d) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
 }
 
-template <int MT>
+template <int MT, int RN>
 __host__ __device__ constexpr int lora_shrink_smem_bytes() {
-  return (8 + 1) * 16 * MT * 64 * 4;  // one partial per warp, their sum
+  return (8 + 1) * 16 * MT * RN * 8 * 4;  // one partial per warp, their sum
 }
 
-// One cluster per 16 MT tokens.  A lane's 16-byte loads hold 8 neighbouring
-// k-values of one row; two mma.sync take them as their k-fragments (the same
-// k-order on both sides, so the dot products are whole).  Only the rows of the
-// adapter at hand are kept, so the partials of all adapters of the tile share
-// one [tokens][64] buffer per warp and are reduced once: over the warps in
-// shared memory, over the cluster through distributed shared memory, in order.
+// Cluster (row tile, w) takes the tile's list entries w, w + walkers, ...: for
+// adapter a_j all rows of H_j, the products of its own tokens and zeros for the
+// others.  The tokens are walked in groups of 16 MT; kc CTAs of the cluster
+// share a group and split its K (all of them for one group, one each for as
+// many groups as CTAs).  A lane's 16-byte loads hold 8 neighbouring k-values of
+// one row; two mma.sync take them as their k-fragments (the same k-order on
+// both sides, so the dot products are whole).  Partial sums meet over the warps
+// in shared memory and over the CTAs through distributed shared memory, in
+// order.
 template <typename T, int MT, int RN>
-__global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const T* x, const T* lora_a,
-                                                                   const LoraArgs args) {
-  constexpr int kTok = 16 * MT;
+__global__ void __launch_bounds__(kLoraThreads, MT == 1 ? 2 : 1) lora_shrink_kernel(const T* x, const T* lora_a,
+                                                                      const LoraArgs args) {
+  constexpr int kTok = 16 * MT, kCols = RN * 8;
   extern __shared__ float sm[];
-  float* part = sm;                  // [8][kTok][64]
-  float* local = sm + 8 * kTok * 64;  // [kTok][64]
-  __shared__ int s_flag[kLoraMaxSlots];  // 1: in use; then its place in the list
-  __shared__ int s_id[kTok], s_uniq[kTok], s_warp[8], s_nuniq;
+  float* part = sm;                      // [8][kTok][kCols]
+  float* local = sm + 8 * kTok * kCols;  // [kTok][kCols]
+  __shared__ int s_flag[kLoraMaxSlots];
+  __shared__ int s_list[kLoraPairRows], s_id[kLoraPairRows], s_rows[kLoraPairRows], s_warp[8];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = args.cluster;
   const int rank = static_cast<int>(cluster_ctarank());
-  const int t0 = static_cast<int>(blockIdx.x) / C * kTok;
-  const int mt = t0 / args.tile_rows, m0 = mt * args.tile_rows;
+  const int cluster = static_cast<int>(blockIdx.x) / C;
+  const int mt = cluster / args.walkers, walker = cluster - mt * args.walkers;
+  const int m0 = mt * args.tile_rows;
+  const int rows = min(args.tile_rows, args.M - m0);  // at most 256, one per thread
   for (int i = tid; i < args.slots; i += kLoraThreads) s_flag[i] = 0;
   cluster_sync();  // every CTA runs before another reads its shared memory
   pdl_wait();
   pdl_allow_next();
-  // The product's row tile: which adapters it uses, in slot order.
-  for (int i = tid; i < args.tile_rows && m0 + i < args.M; i += kLoraThreads) {
-    const int id = args.ids[m0 + i];
-    const bool ok = id >= 0 && id < args.slots && args.ranks[id] > 0;
-    if (ok) s_flag[id] = 1;
-    else if (id != -1 && m0 + i >= t0 && m0 + i < t0 + kTok) report_status(kStatusBadAdapter, m0 + i);
-    if (m0 + i >= t0 && m0 + i < t0 + kTok) s_id[m0 + i - t0] = ok ? id : -1;
+  // Which adapters the row tile uses, in slot order.
+  int my_id = -1;
+  if (tid < rows) {
+    const int id = args.ids[m0 + tid];
+    if (id >= 0 && id < args.slots && args.ranks[id] > 0) {
+      my_id = id;
+      s_flag[id] = 1;
+    } else if (id != -1) {
+      report_status(kStatusBadAdapter, m0 + tid);
+    }
   }
-  for (int i = tid; i < kTok; i += kLoraThreads)
-    if (t0 + i >= args.M) s_id[i] = -1;
+  s_id[tid] = my_id;
   __syncthreads();
   int used[4], mine = 0;
 #pragma unroll
@@ -133,14 +146,6 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const T* x, c
     mine += __popc(b);
   }
   if (lane == 0) s_warp[warp] = mine;
-  if (warp == 0) {  // distinct adapters of this cluster's tokens
-    const int id = lane < kTok ? s_id[lane] : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, id);
-    const bool first = id >= 0 && (same & ((1u << lane) - 1u)) == 0;
-    const unsigned b = __ballot_sync(0xffffffffu, first);
-    if (first) s_uniq[__popc(b & ((1u << lane) - 1u))] = id;
-    if (lane == 0) s_nuniq = __popc(b);
-  }
   __syncthreads();
   int before = 0, total = 0;
 #pragma unroll
@@ -148,96 +153,126 @@ __global__ void __launch_bounds__(kLoraThreads) lora_shrink_kernel(const T* x, c
     before += w < warp ? s_warp[w] : 0;
     total += s_warp[w];
   }
-  const bool writes_list = rank == 0 && t0 == m0;
+  const bool writes_list = rank == 0 && walker == 0;
   if (writes_list && tid == 0) args.count[mt] = total;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (used[i] >= 0) {
       const int slot = warp * 128 + i * 32 + lane;
-      s_flag[slot] = before + used[i];
+      s_list[before + used[i]] = slot;
       if (writes_list) args.list[mt * args.smax + before + used[i]] = slot;
     }
   __syncthreads();
 
   const int g = lane >> 2, q = lane & 3;
-  const int width = 64 * args.parts;
-  T* h = static_cast<T*>(args.h) + static_cast<size_t>(mt) * args.smax * args.tile_rows * width;
-  const T* xr[2 * MT];  // rows g, g + 8, ... of the tile (past M: row 0, dropped below)
+  const T* xt = x + static_cast<size_t>(m0) * args.K;
+  for (int j = walker; j < total; j += args.walkers) {
+    const int id = s_list[j];
+    T* h = static_cast<T*>(args.h) +
+           (static_cast<size_t>(mt) * args.gmax + j * args.rank / 64) * args.tile_rows * 64 +
+           j * args.rank % 64;  // column 0 of the entry; 64 columns on: the next group
+    const size_t group = static_cast<size_t>(args.tile_rows) * 64;
+    // The adapter's tokens, in row order.
+    const bool own = my_id == id;
+    const unsigned b = __ballot_sync(0xffffffffu, own);
+    if (lane == 0) s_warp[warp] = __popc(b);
+    __syncthreads();
+    int at = __popc(b & ((1u << lane) - 1u)), tokens = 0;
 #pragma unroll
-  for (int i = 0; i < 2 * MT; ++i)
-    xr[i] = x + static_cast<size_t>(t0 + 8 * i + g < args.M ? t0 + 8 * i + g : t0) * args.K + q * 8;
-  for (int r0 = 0; r0 < args.rank; r0 += 64) {
-    for (int u = 0; u < s_nuniq; ++u) {
-      const int id = s_uniq[u];
+    for (int w = 0; w < 8; ++w) {
+      at += w < warp ? s_warp[w] : 0;
+      tokens += s_warp[w];
+    }
+    if (own) s_rows[at] = tid;
+    __syncthreads();
+    const int groups = (tokens + kTok - 1) / kTok;
+    int kc = C;
+    while (kc > 1 && C / kc < groups) kc >>= 1;
+    const int sub = rank % kc, lead = rank - sub, stride = C / kc;
+    const int own_rank = args.ranks[id];
+    const float scale = args.scales[id];
+    for (int r0 = 0; r0 < args.rank; r0 += 64) {
       const T* ar = lora_a + (static_cast<size_t>(id) * args.rank + r0 + g) * args.K + q * 8;
-      float acc[MT][RN][4] = {};
-#pragma unroll 2
-      for (int k = (rank * 8 + warp) * 32; k < args.K; k += C * 8 * 32) {
-        const bool in = k + q * 8 < args.K;  // K is a multiple of 8
-        uint4 xa[2 * MT], bv[RN];
+      for (int it = 0; it * stride < groups; ++it) {
+        const int t0 = (it * stride + rank / kc) * kTok;
+        const T* xr[2 * MT];  // rows g, g + 8, ... of the group (past its end: dropped below)
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i)
-          xa[i] = in ? *reinterpret_cast<const uint4*>(xr[i] + k) : make_uint4(0, 0, 0, 0);
+          xr[i] = xt + static_cast<size_t>(s_rows[t0 + 8 * i + g < tokens ? t0 + 8 * i + g : 0]) * args.K + q * 8;
+        float acc[MT][RN][4] = {};
+        if (t0 < tokens) {
+#pragma unroll 2
+          for (int k = (sub * 8 + warp) * 32; k < args.K; k += kc * 8 * 32) {
+            const bool in = k + q * 8 < args.K;  // K is a multiple of 8
+            uint4 xa[2 * MT], bv[RN];
 #pragma unroll
-        for (int n = 0; n < RN; ++n)
-          bv[n] = in ? *reinterpret_cast<const uint4*>(ar + static_cast<size_t>(n) * 8 * args.K + k)
-                     : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 2 * MT; ++i)
+              xa[i] = in ? *reinterpret_cast<const uint4*>(xr[i] + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < RN; ++n)
+              bv[n] = in ? *reinterpret_cast<const uint4*>(ar + static_cast<size_t>(n) * 8 * args.K + k)
+                         : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int n = 0; n < RN; ++n) {
+                mma_16816<T>(acc[m][n], xa[2 * m].x, xa[2 * m + 1].x, xa[2 * m].y, xa[2 * m + 1].y,
+                             bv[n].x, bv[n].y);
+                mma_16816<T>(acc[m][n], xa[2 * m].z, xa[2 * m + 1].z, xa[2 * m].w, xa[2 * m + 1].w,
+                             bv[n].z, bv[n].w);
+              }
+          }
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int n = 0; n < RN; ++n) {
-            mma_16816<T>(acc[m][n], xa[2 * m].x, xa[2 * m + 1].x, xa[2 * m].y, xa[2 * m + 1].y,
-                         bv[n].x, bv[n].y);
-            mma_16816<T>(acc[m][n], xa[2 * m].z, xa[2 * m + 1].z, xa[2 * m].w, xa[2 * m + 1].w,
-                         bv[n].z, bv[n].w);
-          }
-      }
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+            for (int n = 0; n < RN; ++n)
+              *reinterpret_cast<float2*>(part + (warp * kTok + 16 * m + 8 * half + g) * kCols + n * 8 + 2 * q) =
+                  make_float2(acc[m][n][2 * half], acc[m][n][2 * half + 1]);
+        __syncthreads();
+        for (int i = tid; i < kTok * kCols; i += kLoraThreads) {
+          const int row = i / kCols, c = i % kCols;
+          float sum = 0.f;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int row = 16 * m + 8 * half + g;
-          if (s_id[row] != id) continue;
-#pragma unroll
-          for (int n = 0; n < RN; ++n)
-            *reinterpret_cast<float2*>(part + (warp * kTok + row) * 64 + n * 8 + 2 * q) =
-                make_float2(acc[m][n][2 * half], acc[m][n][2 * half + 1]);
+          for (int w = 0; w < 8; ++w) sum += part[(w * kTok + row) * kCols + c];
+          local[row * kCols + c] = sum;
         }
-    }
-    __syncthreads();
-    constexpr int kCols = RN * 8;
-    for (int i = tid; i < kTok * kCols; i += kLoraThreads) {
-      const int row = i / kCols, c = i % kCols;
-      float sum = 0.f;
-      if (s_id[row] >= 0) {
-#pragma unroll
-        for (int w = 0; w < 8; ++w) sum += part[(w * kTok + row) * 64 + c];
+        if (kc > 1) cluster_sync();
+        else __syncthreads();
+        for (int i = sub * kLoraThreads + tid; i < kTok * kCols / 2; i += kc * kLoraThreads) {
+          const int row = i / (kCols / 2), c = i % (kCols / 2) * 2;
+          if (t0 + row >= tokens) continue;
+          float2 sum = make_float2(0.f, 0.f);
+          if (kc > 1) {
+            const uint32_t a = smem_addr(local + row * kCols + c);
+            for (int p = 0; p < kc; ++p) {
+              const float2 v = ld_cluster_f32x2(map_shared(a, lead + p));
+              sum.x += v.x;
+              sum.y += v.y;
+            }
+          } else {
+            sum = *reinterpret_cast<const float2*>(local + row * kCols + c);
+          }
+          // Past the adapter's own rank H is 0 whatever x holds.
+          sum.x = r0 + c < own_rank ? sum.x * scale : 0.f;
+          sum.y = r0 + c + 1 < own_rank ? sum.y * scale : 0.f;
+          *reinterpret_cast<uint32_t*>(h + r0 / 64 * group + s_rows[t0 + row] * 64 + c) =
+              Pack2<T>::pack(sum.x, sum.y);
+        }
+        // The sums are read before the next ones overwrite them, or the CTA leaves.
+        if (kc > 1) cluster_sync();
+        else __syncthreads();
       }
-      local[row * 64 + c] = sum;
     }
-    cluster_sync();
-    for (int i = rank * kLoraThreads + tid; i < kTok * kCols; i += C * kLoraThreads) {
-      const int row = i / kCols, c = i % kCols;
-      const int id = s_id[row];
-      if (id < 0) continue;
-      const uint32_t at = smem_addr(local + row * 64 + c);
-      float sum = 0.f;
-      for (int p = 0; p < C; ++p) sum += ld_cluster_f32(map_shared(at, p));
-      // Past the adapter's own rank H is 0 whatever x holds.
-      const float v = r0 + c < args.ranks[id] ? sum * args.scales[id] : 0.f;
-      h[(static_cast<size_t>(s_flag[id]) * args.tile_rows + t0 - m0 + row) * width + r0 + c] =
-          Pack2<T>::from_float(v);
+    // Zeros where the tile's other tokens meet this adapter.
+    const int vecs = args.rank / 8;
+    for (int i = rank * kLoraThreads + tid; i < rows * vecs; i += C * kLoraThreads) {
+      const int row = i / vecs, c = (i - row * vecs) * 8;
+      if (s_id[row] != id)
+        *reinterpret_cast<uint4*>(h + c / 64 * group + row * 64 + c % 64) = make_uint4(0, 0, 0, 0);
     }
-    cluster_sync();  // sums read before the next part overwrites them, or the CTA leaves
-  }
-  // Zeros where a token meets another adapter of its row tile.
-  const int vecs = args.rank / 8;
-  for (int i = rank * kLoraThreads + tid; i < kTok * total * vecs; i += C * kLoraThreads) {
-    const int v = i % vecs, e = i / vecs % total, row = i / (vecs * total);
-    if (t0 + row >= args.M || (s_id[row] >= 0 && s_flag[s_id[row]] == e)) continue;
-    *reinterpret_cast<uint4*>(
-        h + (static_cast<size_t>(e) * args.tile_rows + t0 - m0 + row) * width + v * 8) =
-        make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -252,7 +287,7 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
 }
 
 __host__ __device__ inline int lora_stream_smem_bytes(int nt, int stages) {
-  return 1024 + stages * (kMdStageW + nt * 256) + (2 * stages + 1) * 8 + 16;
+  return 1024 + stages * (kMdStageW + nt * 256) + (2 * stages + 2) * 8 + 16 + kLoraPairRows * 4;
 }
 
 // 128 columns x tile_rows tokens per cluster of C CTAs.  CTA r runs the k-steps
@@ -276,15 +311,18 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(sB + stages * stage_b);
   uint64_t* empty = full + stages;
   uint64_t* tfull = empty + stages;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tfull + 1);
+  uint64_t* listed = tfull + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(listed + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  volatile int* s_width = reinterpret_cast<volatile int*>(tmem_holder + 2);
+  volatile int* s_slot = reinterpret_cast<volatile int*>(tmem_holder + 4);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const int tile = static_cast<int>(blockIdx.x) / C;
   const int chunk = tile % args.chunks, n0 = tile / args.chunks * 128;
   const int ksteps = (args.K + 127) / 128;
   const int kb0 = rank * ksteps / C, kb1 = (rank + 1) * ksteps / C;
-  const int rs = min(args.rank, 64);  // k-values of one list step
+  const int R = args.rank, rs = min(R, 64);  // rs: rows of B in one box
   uint32_t tmem_cols = 32;
   while (tmem_cols < static_cast<uint32_t>(nt)) tmem_cols *= 2;
 
@@ -294,6 +332,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
       mbar_init(&empty[s], 1);
     }
     mbar_init(tfull, 1);
+    mbar_init(listed, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_w);
@@ -311,15 +350,16 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
 
-  // The entries of this CTA's share of the row tile's list: known once the
-  // shrink kernel is done.
-  auto entries = [&](int* e0) {
+  // This CTA's share of the row tile's list, known once the shrink kernel is
+  // done: warp 3 brings the slots into shared memory in one round of loads.
+  if (warp == 3) {
     pdl_wait();
     const int n = __ldcg(args.count + chunk);
-    *e0 = rank * n / C;
-    return (rank + 1) * n / C;
-  };
-
+    for (int i = lane; i < n; i += 32) s_slot[i] = __ldcg(args.list + chunk * args.smax + i);
+    if (lane == 0) *s_width = n * R;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(listed);
+  }
   if (warp == 0) {
     if (elect_one()) {
       int stage = 0;
@@ -338,16 +378,18 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
           phase ^= 1u;
         }
       }
-      int e0, e1 = 0;
-      if (ok) e1 = entries(&e0);
-      for (int i = ok ? e0 * args.parts : 0; i < e1 * args.parts; ++i) {
-        const int slot = __ldcg(args.list + chunk * args.smax + i / args.parts);
+      if (ok) ok = mbar_wait(listed, 0, abort_flag, 57);
+      const int cols = ok ? *s_width : 0, groups = (cols + 63) / 64;
+      for (int i = rank * groups / C; i < (rank + 1) * groups / C; ++i) {
         if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, 52)) break;
         uint8_t* w = sW + stage * kMdStageW;
-        const int row = i % args.parts * 64;
-        mbar_arrive_expect_tx(&full[stage], 2 * rs * 128);
-        tma_load_3d(w, &tm_b, &full[stage], n0, row, slot);
-        tma_load_3d(w + 8192, &tm_b, &full[stage], n0 + 64, row, slot);
+        const int c1 = min(cols, i * 64 + 64);
+        mbar_arrive_expect_tx(&full[stage], (c1 - i * 64) * 256);
+        for (int c = i * 64; c < c1; c += rs, w += rs * 128) {
+          const int slot = s_slot[c / R];
+          tma_load_3d(w, &tm_b, &full[stage], n0, c % R, slot);
+          tma_load_3d(w + 8192, &tm_b, &full[stage], n0 + 64, c % R, slot);
+        }
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
@@ -370,14 +412,14 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
           phase ^= 1u;
         }
       }
-      int e0, e1 = 0;
-      if (ok) e1 = entries(&e0);
+      if (ok) ok = mbar_wait(listed, 0, abort_flag, 58);
+      const int cols = ok ? *s_width : 0, groups = (cols + 63) / 64;
+      pdl_wait();
       fence_proxy_async_all();  // H was stored by ordinary stores
-      for (int i = ok ? e0 * args.parts : 0; i < e1 * args.parts; ++i) {
+      for (int i = rank * groups / C; i < (rank + 1) * groups / C; ++i) {
         if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, 54)) break;
         mbar_arrive_expect_tx(&full[stage], nt * 128);
-        tma_load_2d(sB + stage * stage_b, &tm_h, &full[stage], i % args.parts * 64,
-                    (chunk * args.smax + i / args.parts) * nt);
+        tma_load_2d(sB + stage * stage_b, &tm_h, &full[stage], 0, (chunk * args.gmax + i) * nt);
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
@@ -410,9 +452,10 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
         return true;
       };
       for (int kb = kb0; ok && kb < kb1; ++kb) ok = step(8);
-      int e0, e1 = 0;
-      if (ok) e1 = entries(&e0);
-      for (int i = ok ? e0 * args.parts : 0; ok && i < e1 * args.parts; ++i) ok = step(rs / 16);
+      if (ok) ok = mbar_wait(listed, 0, abort_flag, 59);
+      const int cols = ok ? *s_width : 0, groups = (cols + 63) / 64;
+      for (int i = rank * groups / C; ok && i < (rank + 1) * groups / C; ++i)
+        ok = step(min(64, cols - i * 64) / 16);
       if (ok) umma_commit(tfull);
     }
   }
@@ -427,7 +470,8 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
   }
   __syncthreads();
   cluster_sync();  // every CTA of the cluster has consumed its ring
-  float* recv = reinterpret_cast<float*>(sW);  // [C sources][tokens of this rank][128]
+  // [C sources][tokens of this rank / 4][128 columns][4 tokens]
+  float* recv = reinterpret_cast<float*>(sW);
   const int own = nt / C;
   if (warp >= 4 && __all_sync(0xffffffffu, ok)) {
     tc_fence_after();
@@ -437,10 +481,10 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
       tmem_ld_32x32b_x16(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + c, v);
       tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < 16; j += 4) {
         const int to = (c + j) / own;
-        const uint32_t at = smem_addr(recv + (rank * own + (c + j - to * own)) * 128 + q * 32 + lane);
-        st_cluster_f32(map_shared(at, to), __uint_as_float(v[j]));
+        const uint32_t at = smem_addr(recv + (rank * own + (c + j - to * own)) * 128 + (q * 32 + lane) * 4);
+        st_cluster_u32x4(map_shared(at, to), v[j], v[j + 1], v[j + 2], v[j + 3]);
       }
     }
     tc_fence_before();
@@ -448,17 +492,22 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
   cluster_sync();
   T* out = static_cast<T*>(args.out);
   const int row0 = chunk * nt + rank * own;
-  for (int i = threadIdx.x; i < own * 64; i += kLoraThreads) {
-    const int tok = i >> 6, c = (i & 63) * 2;
+  for (int i = threadIdx.x; i < own * 16; i += kLoraThreads) {
+    const int tok = (i >> 6) * 4, c = (i & 63) * 2;
     if (row0 + tok >= args.M || n0 + c >= args.N) continue;
-    float2 sum = make_float2(0.f, 0.f);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;  // four tokens of columns c, c + 1
     for (int s = 0; s < C; ++s) {
-      const float2 v = *reinterpret_cast<const float2*>(recv + (s * own + tok) * 128 + c);
-      sum.x += v.x;
-      sum.y += v.y;
+      const float4* p = reinterpret_cast<const float4*>(recv + (s * own + tok) * 128 + c * 4);
+      const float4 va = p[0], vb = p[1];
+      a.x += va.x, a.y += va.y, a.z += va.z, a.w += va.w;
+      b.x += vb.x, b.y += vb.y, b.z += vb.z, b.w += vb.w;
     }
-    *reinterpret_cast<uint32_t*>(out + static_cast<size_t>(row0 + tok) * args.N + n0 + c) =
-        Pack2<T>::pack(sum.x, sum.y);
+    const uint32_t pk[4] = {Pack2<T>::pack(a.x, b.x), Pack2<T>::pack(a.y, b.y),
+                            Pack2<T>::pack(a.z, b.z), Pack2<T>::pack(a.w, b.w)};
+    T* o = out + static_cast<size_t>(row0 + tok) * args.N + n0 + c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (row0 + tok + j < args.M) *reinterpret_cast<uint32_t*>(o + static_cast<size_t>(j) * args.N) = pk[j];
   }
   __syncthreads();
   if (warp == 3) {
@@ -473,8 +522,8 @@ __host__ __device__ inline int lora_tc2_smem_bytes(int stages) {
 
 // The dense CTA-pair GEMM (gemm_tc2.cuh: 256 x 256 pair tiles, GROUP_M raster,
 // two accumulators) with the row tile's adapters appended to each tile's K
-// loop: per list entry, 128 rows of H and `rank` rows of B per CTA.  Tensor
-// bound: an entry costs rank / 64 of a k-step.
+// loop: per 64 columns of H, 128 of its rows and 64 rows of B per CTA.  Tensor
+// bound: an adapter costs R / 64 of a k-step.
 template <typename T>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     lora_tc2_kernel(const __grid_constant__ CUtensorMap tm_x,
@@ -504,7 +553,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int nm = (M + kLoraPairRows - 1) / kLoraPairRows, nn = (N + BN - 1) / BN;
   const int ntiles = nm * nn;
   const int nkb = (args.K + kGemmBK - 1) / kGemmBK;
-  const int rs = min(args.rank, 64);
+  const int R = args.rank, rs = min(R, 64);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
@@ -571,17 +620,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           pdl_wait();
           fence_proxy_async_all();  // H was stored by ordinary stores
         }
-        const int steps = __ldcg(args.count + pm) * args.parts;
-        for (int e = 0; e < steps; ++e) {
-          const int entry = pm * args.smax + e / args.parts;
-          const int slot = __ldcg(args.list + entry), part = e % args.parts * 64;
+        const int cols = __ldcg(args.count + pm) * R;
+        int next = __ldcg(args.list + pm * args.smax);
+        for (int c0 = 0; c0 < cols; c0 += 64) {
           if (!(ok = mbar_wait_cluster(&empty[stage], phase ^ 1u, abort_flag, 62))) break;
           const uint32_t bar = map_shared(smem_addr(&full[stage]), 0);
-          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * (kGemmABytes + 2 * rs * 128));
-          tma_load_2d_pair(sA + stage * kGemmABytes, &tm_h, bar, part,
-                           entry * kLoraPairRows + rank * kGemmBM);
-          tma_load_3d_pair(sB + stage * Shape::kBBytes, &tm_b, bar, col, part, slot);
-          tma_load_3d_pair(sB + stage * Shape::kBBytes + 8192, &tm_b, bar, col + 64, part, slot);
+          const int c1 = min(cols, c0 + 64);
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * (kGemmABytes + (c1 - c0) * 256));
+          tma_load_2d_pair(sA + stage * kGemmABytes, &tm_h, bar, 0,
+                           (pm * args.gmax + c0 / 64) * kLoraPairRows + rank * kGemmBM);
+          uint8_t* b = sB + stage * Shape::kBBytes;
+          for (int c = c0; c < c1; c += rs, b += rs * 128) {
+            const int slot = next;
+            if (c + rs < cols) next = __ldcg(args.list + pm * args.smax + (c + rs) / R);
+            tma_load_3d_pair(b, &tm_b, bar, col, c % R, slot);
+            tma_load_3d_pair(b + 8192, &tm_b, bar, col + 64, c % R, slot);
+          }
           if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
@@ -621,8 +675,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         for (int kb = 0; ok && kb < nkb; ++kb) ok = step(4, kb == 0);
         if (!ok) break;
         if (i == 0) pdl_wait();
-        const int steps = __ldcg(args.count + pm) * args.parts;
-        for (int e = 0; ok && e < steps; ++e) ok = step(rs / 16, false);
+        const int cols = __ldcg(args.count + pm) * R;
+        for (int c = 0; ok && c < cols; c += 64) ok = step(min(64, cols - c) / 16, false);
         if (ok) umma_commit_both(&tfull[acc]);
       }
     }
