@@ -142,6 +142,23 @@ int ensure_smem(const void* fn, int bytes) {
   return BOKT_OK;
 }
 
+// Ask for the largest shared-memory carve-out for a small kernel whose successor
+// is launched while it runs: the successor's CTAs only join an SM whose carve-out
+// already holds them.  Once per (device, kernel).
+int ensure_carveout(const void* fn) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(g_smem_mu);
+  for (int i = 0; i < g_smem_attr_n; ++i)
+    if (g_smem_attr[i].dev == dev && g_smem_attr[i].fn == fn && g_smem_attr[i].bytes == -1)
+      return BOKT_OK;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                       cudaSharedmemCarveoutMaxShared);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(PreferredSharedMemoryCarveout)");
+  if (g_smem_attr_n < 512) g_smem_attr[g_smem_attr_n++] = {dev, fn, -1};
+  return BOKT_OK;
+}
+
 // ----------------------------------------------------------------- tensor maps
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
@@ -1824,6 +1841,7 @@ int bokt_moe_decode(const void* x, const void* logits, int logits_dtype, const v
     attr[lc.numAttrs].val.clusterDim.y = 1;
     attr[lc.numAttrs].val.clusterDim.z = 1;
     lc.numAttrs += 1;
+    if ((rc = ensure_carveout(fn))) return rc;
     int renorm = renormalize ? 1 : 0;
     void* kargs[] = {const_cast<void*>(static_cast<const void*>(&logits)), &renorm, &a};
     cudaError_t e = cudaLaunchKernelExC(&lc, fn, kargs);
@@ -2057,12 +2075,13 @@ int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void*
                                             : lora_shrink_ptr<__half, 2>(rank, &smem))
                                       : (bf ? lora_shrink_ptr<__nv_bfloat16, 1>(rank, &smem)
                                             : lora_shrink_ptr<__half, 1>(rank, &smem));
-    if ((rc = ensure_smem(fn, smem))) return rc;
+    if ((rc = ensure_smem(fn, smem)) || (rc = ensure_carveout(fn))) return rc;
     const int clusters = p.tiles * p.walkers;
     a.cluster = p.shrink_cluster;
     a.walkers = p.walkers;
     void* kargs[] = {&x, &lora_a, &a};
-    cudaError_t e = launch_cluster(fn, clusters * a.cluster, bokt::kLoraThreads, smem, a.cluster, s, kargs);
+    const int threads = 32 * (p.shrink_mt == 2 ? bokt::lora_shrink_warps<2>() : bokt::lora_shrink_warps<1>());
+    cudaError_t e = launch_cluster(fn, clusters * a.cluster, threads, smem, a.cluster, s, kargs);
     if (e != cudaSuccess) return cuda_fail(e, "lora_shrink launch");
   }
   a.cluster = p.cluster;

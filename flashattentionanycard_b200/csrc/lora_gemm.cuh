@@ -90,9 +90,15 @@ __device__ __forceinline__ void st_cluster_u32x4(uint32_t addr, uint32_t a, uint
                : "memory");
 }
 
+// Row tiles of many tokens (MT = 2) have few clusters to hide latency with:
+// twice the warps.
+template <int MT>
+__host__ __device__ constexpr int lora_shrink_warps() {
+  return MT == 1 ? 8 : 16;
+}
 template <int MT, int RN>
 __host__ __device__ constexpr int lora_shrink_smem_bytes() {
-  return (8 + 1) * 16 * MT * RN * 8 * 4;  // one partial per warp, their sum
+  return (lora_shrink_warps<MT>() + 1) * 16 * MT * RN * 8 * 4;  // a partial per warp, their sum
 }
 
 // Cluster (row tile, w) takes the tile's list entries w, w + walkers, ...: for
@@ -105,14 +111,16 @@ __host__ __device__ constexpr int lora_shrink_smem_bytes() {
 // in shared memory and over the CTAs through distributed shared memory, in
 // order.
 template <typename T, int MT, int RN>
-__global__ void __launch_bounds__(kLoraThreads, MT == 1 ? 2 : 1) lora_shrink_kernel(const T* x, const T* lora_a,
-                                                                      const LoraArgs args) {
+__global__ void __launch_bounds__(32 * lora_shrink_warps<MT>(), MT == 1 ? 2 : 1)
+    lora_shrink_kernel(const T* x, const T* lora_a, const LoraArgs args) {
   constexpr int kTok = 16 * MT, kCols = RN * 8;
+  constexpr int NW = lora_shrink_warps<MT>(), kThreads = 32 * NW;
+  constexpr int kVotes = kLoraMaxSlots / kThreads;  // slots per lane
   extern __shared__ float sm[];
-  float* part = sm;                      // [8][kTok][kCols]
-  float* local = sm + 8 * kTok * kCols;  // [kTok][kCols]
+  float* part = sm;                      // [NW][kTok][kCols]
+  float* local = sm + NW * kTok * kCols;  // [kTok][kCols]
   __shared__ int s_flag[kLoraMaxSlots];
-  __shared__ int s_list[kLoraPairRows], s_id[kLoraPairRows], s_rows[kLoraPairRows], s_warp[8];
+  __shared__ int s_list[kLoraPairRows], s_id[kLoraPairRows], s_rows[kLoraPairRows], s_warp[NW];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = args.cluster;
   const int rank = static_cast<int>(cluster_ctarank());
@@ -120,7 +128,7 @@ __global__ void __launch_bounds__(kLoraThreads, MT == 1 ? 2 : 1) lora_shrink_ker
   const int mt = cluster / args.walkers, walker = cluster - mt * args.walkers;
   const int m0 = mt * args.tile_rows;
   const int rows = min(args.tile_rows, args.M - m0);  // at most 256, one per thread
-  for (int i = tid; i < args.slots; i += kLoraThreads) s_flag[i] = 0;
+  for (int i = tid; i < args.slots; i += kThreads) s_flag[i] = 0;
   cluster_sync();  // every CTA runs before another reads its shared memory
   pdl_wait();
   pdl_allow_next();
@@ -135,12 +143,12 @@ __global__ void __launch_bounds__(kLoraThreads, MT == 1 ? 2 : 1) lora_shrink_ker
       report_status(kStatusBadAdapter, m0 + tid);
     }
   }
-  s_id[tid] = my_id;
+  if (tid < kLoraPairRows) s_id[tid] = my_id;
   __syncthreads();
-  int used[4], mine = 0;
+  int used[kVotes], mine = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int slot = warp * 128 + i * 32 + lane;
+  for (int i = 0; i < kVotes; ++i) {
+    const int slot = warp * 32 * kVotes + i * 32 + lane;
     const unsigned b = __ballot_sync(0xffffffffu, slot < args.slots && s_flag[slot]);
     used[i] = b >> lane & 1u ? mine + __popc(b & ((1u << lane) - 1u)) : -1;
     mine += __popc(b);
@@ -149,16 +157,16 @@ __global__ void __launch_bounds__(kLoraThreads, MT == 1 ? 2 : 1) lora_shrink_ker
   __syncthreads();
   int before = 0, total = 0;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
+  for (int w = 0; w < NW; ++w) {
     before += w < warp ? s_warp[w] : 0;
     total += s_warp[w];
   }
   const bool writes_list = rank == 0 && walker == 0;
   if (writes_list && tid == 0) args.count[mt] = total;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < kVotes; ++i)
     if (used[i] >= 0) {
-      const int slot = warp * 128 + i * 32 + lane;
+      const int slot = warp * 32 * kVotes + i * 32 + lane;
       s_list[before + used[i]] = slot;
       if (writes_list) args.list[mt * args.smax + before + used[i]] = slot;
     }
@@ -179,7 +187,7 @@ __global__ void __launch_bounds__(kLoraThreads, MT == 1 ? 2 : 1) lora_shrink_ker
     __syncthreads();
     int at = __popc(b & ((1u << lane) - 1u)), tokens = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < NW; ++w) {
       at += w < warp ? s_warp[w] : 0;
       tokens += s_warp[w];
     }
@@ -202,7 +210,7 @@ __global__ void __launch_bounds__(kLoraThreads, MT == 1 ? 2 : 1) lora_shrink_ker
         float acc[MT][RN][4] = {};
         if (t0 < tokens) {
 #pragma unroll 2
-          for (int k = (sub * 8 + warp) * 32; k < args.K; k += kc * 8 * 32) {
+          for (int k = (sub * NW + warp) * 32; k < args.K; k += kc * NW * 32) {
             const bool in = k + q * 8 < args.K;  // K is a multiple of 8
             uint4 xa[2 * MT], bv[RN];
 #pragma unroll
@@ -232,16 +240,16 @@ __global__ void __launch_bounds__(kLoraThreads, MT == 1 ? 2 : 1) lora_shrink_ker
               *reinterpret_cast<float2*>(part + (warp * kTok + 16 * m + 8 * half + g) * kCols + n * 8 + 2 * q) =
                   make_float2(acc[m][n][2 * half], acc[m][n][2 * half + 1]);
         __syncthreads();
-        for (int i = tid; i < kTok * kCols; i += kLoraThreads) {
+        for (int i = tid; i < kTok * kCols; i += kThreads) {
           const int row = i / kCols, c = i % kCols;
           float sum = 0.f;
 #pragma unroll
-          for (int w = 0; w < 8; ++w) sum += part[(w * kTok + row) * kCols + c];
+          for (int w = 0; w < NW; ++w) sum += part[(w * kTok + row) * kCols + c];
           local[row * kCols + c] = sum;
         }
         if (kc > 1) cluster_sync();
         else __syncthreads();
-        for (int i = sub * kLoraThreads + tid; i < kTok * kCols / 2; i += kc * kLoraThreads) {
+        for (int i = sub * kThreads + tid; i < kTok * kCols / 2; i += kc * kThreads) {
           const int row = i / (kCols / 2), c = i % (kCols / 2) * 2;
           if (t0 + row >= tokens) continue;
           float2 sum = make_float2(0.f, 0.f);
@@ -268,7 +276,7 @@ __global__ void __launch_bounds__(kLoraThreads, MT == 1 ? 2 : 1) lora_shrink_ker
     }
     // Zeros where the tile's other tokens meet this adapter.
     const int vecs = args.rank / 8;
-    for (int i = rank * kLoraThreads + tid; i < rows * vecs; i += C * kLoraThreads) {
+    for (int i = rank * kThreads + tid; i < rows * vecs; i += C * kThreads) {
       const int row = i / vecs, c = (i - row * vecs) * 8;
       if (s_id[row] != id)
         *reinterpret_cast<uint4*>(h + c / 64 * group + row * 64 + c % 64) = make_uint4(0, 0, 0, 0);
@@ -287,7 +295,7 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
 }
 
 __host__ __device__ inline int lora_stream_smem_bytes(int nt, int stages) {
-  return 1024 + stages * (kMdStageW + nt * 256) + (2 * stages + 2) * 8 + 16 + kLoraPairRows * 4;
+  return 1024 + stages * (kMdStageW + nt * 256) + (2 * stages + 3) * 8 + 16 + kLoraPairRows * 4;
 }
 
 // 128 columns x tile_rows tokens per cluster of C CTAs.  CTA r runs the k-steps
@@ -312,7 +320,8 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
   uint64_t* empty = full + stages;
   uint64_t* tfull = empty + stages;
   uint64_t* listed = tfull + 1;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(listed + 1);
+  uint64_t* issued = listed + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(issued + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   volatile int* s_width = reinterpret_cast<volatile int*>(tmem_holder + 2);
   volatile int* s_slot = reinterpret_cast<volatile int*>(tmem_holder + 4);
@@ -333,6 +342,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
     }
     mbar_init(tfull, 1);
     mbar_init(listed, 1);
+    mbar_init(issued, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_w);
@@ -378,18 +388,14 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
           phase ^= 1u;
         }
       }
-      if (ok) ok = mbar_wait(listed, 0, abort_flag, 57);
+      if (ok) {
+        mbar_arrive(issued);
+        ok = mbar_wait(listed, 0, abort_flag, 57);
+      }
       const int cols = ok ? *s_width : 0, groups = (cols + 63) / 64;
       for (int i = rank * groups / C; i < (rank + 1) * groups / C; ++i) {
         if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, 52)) break;
-        uint8_t* w = sW + stage * kMdStageW;
-        const int c1 = min(cols, i * 64 + 64);
-        mbar_arrive_expect_tx(&full[stage], (c1 - i * 64) * 256);
-        for (int c = i * 64; c < c1; c += rs, w += rs * 128) {
-          const int slot = s_slot[c / R];
-          tma_load_3d(w, &tm_b, &full[stage], n0, c % R, slot);
-          tma_load_3d(w + 8192, &tm_b, &full[stage], n0 + 64, c % R, slot);
-        }
+        mbar_arrive_expect_tx(&full[stage], min(64, cols - i * 64) * 256);  // from warps 4-7
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
@@ -459,6 +465,26 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
       if (ok) umma_commit(tfull);
     }
   }
+  if (warp >= 4) {
+    // The B rows of a 64-deep step: up to four adapters of two boxes each, one
+    // adapter per warp (issued by one thread they take longer than to arrive).
+    // A parity wait tells neighbouring uses of a stage apart only, so these
+    // start when warp 0 has issued, and so waited for, every k-step before them.
+    if (elect_one() && mbar_wait(listed, 0, abort_flag, 60) && mbar_wait(issued, 0, abort_flag, 62)) {
+      const int cols = *s_width, groups = (cols + 63) / 64;
+      const int g0 = rank * groups / C, g1 = (rank + 1) * groups / C;
+      for (int i = g0; i < g1; ++i) {
+        const int c = i * 64 + (warp - 4) * rs;
+        if ((warp - 4) * rs >= 64 || c >= cols) break;
+        const int step = kb1 - kb0 + i - g0, stage = step % stages;
+        if (!mbar_wait(&empty[stage], (step / stages & 1) ^ 1, abort_flag, 61)) break;
+        uint8_t* w = sW + stage * kMdStageW + (warp - 4) * rs * 128;
+        const int slot = s_slot[c / R];
+        tma_load_3d(w, &tm_b, &full[stage], n0, c % R, slot);
+        tma_load_3d(w + 8192, &tm_b, &full[stage], n0 + 64, c % R, slot);
+      }
+    }
+  }
   __syncwarp();
   const bool ok = mbar_wait(tfull, 0, abort_flag, 56);
   pdl_wait();
@@ -476,15 +502,21 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
   if (warp >= 4 && __all_sync(0xffffffffu, ok)) {
     tc_fence_after();
     const int q = warp & 3;
+    const uint32_t mine = smem_addr(recv + rank * own * 128 + (q * 32 + lane) * 4);
+    uint32_t to = 0, at = map_shared(mine, 0), left = own;
     for (int c = 0; c < nt; c += 16) {
       uint32_t v[16];
       tmem_ld_32x32b_x16(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + c, v);
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 16; j += 4) {
-        const int to = (c + j) / own;
-        const uint32_t at = smem_addr(recv + (rank * own + (c + j - to * own)) * 128 + (q * 32 + lane) * 4);
-        st_cluster_u32x4(map_shared(at, to), v[j], v[j + 1], v[j + 2], v[j + 3]);
+        st_cluster_u32x4(at, v[j], v[j + 1], v[j + 2], v[j + 3]);
+        at += 4 * 128 * 4;
+        left -= 4;
+        if (left == 0 && c + j + 4 < nt) {
+          at = map_shared(mine, ++to);
+          left = own;
+        }
       }
     }
     tc_fence_before();
