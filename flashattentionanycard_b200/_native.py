@@ -203,25 +203,56 @@ def dtype_code(dtype):
 
 
 def current_stream(device):
-    """Handle of torch's current stream on a tensor's device (without building
-    the Stream object, which costs more than a decode kernel runs)."""
+    """Handle of torch's current stream on a device (or device index), without
+    building the Stream object, which costs more than a decode kernel runs."""
     import torch
 
-    index = torch.cuda.current_device() if device.index is None else device.index
+    index = device if isinstance(device, int) else device.index
+    if index is None:
+        index = torch.cuda.current_device()
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
 
 
 _SAME_DEVICE = contextlib.nullcontext()
 
 
-def on_device(device):
-    """Context in which ``device`` (a tensor's) is the current CUDA device; the
-    library launches on the current one.  Free of cost where it already is."""
+def on_device(index):
+    """Context in which device ``index`` (a tensor's) is the current CUDA device;
+    the library launches on the current one.  Free of cost where it already is."""
     import torch
 
-    if torch.cuda.current_device() == device.index:
+    if torch._C._cuda_getDevice() == index:
         return _SAME_DEVICE
-    return torch.cuda.device(device)
+    return torch.cuda.device(index)
+
+
+_workspace_need = {}
+
+
+def workspace(entry, sizes, index, given):
+    """(tensor, bytes) of scratch for one call: ``given``, checked, or a fresh
+    tensor from torch's allocator (so that calls on other streams and other
+    captured graphs each have their own).  ``entry`` is the library's
+    ..._workspace_bytes function and ``sizes`` its arguments; device ``index``
+    must be current."""
+    import torch
+
+    key = (entry, sizes, index)
+    need = _workspace_need.get(key)
+    if need is None:
+        lib = load()
+        need = int(getattr(lib, entry)(*sizes))
+        if need < 0:
+            raise RuntimeError(f"{entry}: {lib.bokt_last_error().decode(errors='replace')}")
+        if len(_workspace_need) >= 4096:
+            _workspace_need.clear()
+        _workspace_need[key] = need
+    if given is None:
+        return torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index)), need
+    have = given.numel() * given.element_size()
+    if given.get_device() != index or not given.is_contiguous() or have < need:
+        raise ValueError(f"workspace must be a contiguous tensor of {need} bytes on cuda:{index}")
+    return given, have
 
 
 def device_status(reset=True):

@@ -53,6 +53,9 @@ constexpr int kMdMaxStages = 8;
 // spreading saves (one token, 8 experts x [1024, 2 x 2048]: 29.2 us a call with 1,
 // 24.2 with 4, 25.8 with 8).
 constexpr int kMdMinSteps = 4;
+// Phase 1 cuts tiles only where that shortens the longest share by more k-steps
+// than the cut tiles' way through memory takes.
+constexpr int kMdSplitSteps = 12;
 
 // Header words of the workspace.
 constexpr int kMdClaim = 0, kMdDone1 = 32, kMdDone2 = 64, kMdActive = 96, kMdCount1 = 128;
@@ -261,6 +264,7 @@ struct MdPlan {
   int active;                          // experts in use
   int tiles1, steps1, units1, shares1;  // per expert: tiles1 of 128 + 128 columns
   int tiles2, steps2, units2, shares2;  // tiles2 column blocks of 256, experts inside
+  int whole1;                          // phase 1 shares end at tile ends
   int claims;                          // of all phases
   const int* act_e;
   const int* act_off;
@@ -284,8 +288,13 @@ __device__ __forceinline__ MdSegments md_segments(const MdPlan& p, int phase, in
   const int units = phase == 0 ? p.units1 : p.units2;
   const int shares = phase == 0 ? p.shares1 : p.shares2;
   s.steps = phase == 0 ? p.steps1 : p.steps2;
-  s.u = md_share_begin(share, units, shares);
-  s.u1 = md_share_begin(share + 1, units, shares);
+  if (phase == 0 && p.whole1) {
+    s.u = md_share_begin(share, units / s.steps, shares) * s.steps;
+    s.u1 = md_share_begin(share + 1, units / s.steps, shares) * s.steps;
+  } else {
+    s.u = md_share_begin(share, units, shares);
+    s.u1 = md_share_begin(share + 1, units, shares);
+  }
   return s;
 }
 
@@ -335,47 +344,63 @@ struct MdCols {
   }
 };
 
+// What lane j knows of a token's j-th expert for one column block of phase 3.
+struct MdSlot {
+  int row = 0, base = 0;  // packed row, and its place among its expert's rows
+  int g0 = 0, g1 = -1;    // shares that begin inside its tile: partials to add
+  float gate = 0.f;
+  __device__ __forceinline__ void load(const MoeDecodeArgs& args, const MdPlan& plan, int t, int nb,
+                                       int lane) {
+    if (lane >= args.topk) return;
+    const int as = t * args.topk + lane;
+    row = args.row_of[as];
+    gate = args.gates[as];
+    const int a = args.act_of[as];
+    base = row - plan.act_off[a];
+    const int u = (nb * plan.active + a) * plan.steps2;
+    g0 = md_share_of(u, plan.units2, plan.shares2) + 1;
+    g1 = md_share_of(u + plan.steps2 - 1, plan.units2, plan.shares2);
+  }
+};
+
 // Items first, first + stride, ... of phase 3: the gate-weighted sum of one
 // token's rows of y over 32 CPL columns, each row completed by the partials of
 // the shares that begin inside its tile.  All rows are loaded before the first
-// is used; the sum runs in slot order.
+// is used; the sum runs in slot order.  The first item's slots are read before
+// the wait for phase 2.
 template <typename T, int CPL>
-__device__ __forceinline__ void md_combine(const MoeDecodeArgs& args, const MdPlan& plan, int first,
-                                           int stride, int lane) {
+__device__ __forceinline__ bool md_combine(const MoeDecodeArgs& args, const MdPlan& plan, int first,
+                                           int stride, int lane, volatile int* abort_flag) {
   const int K = args.k, topk = args.topk;
   const int blocks = (K + 32 * CPL - 1) / (32 * CPL);
   const size_t slot_floats = static_cast<size_t>(args.tokens) * 256;
   using Vec = MdCols<CPL>;
+  bool waited = false;
   for (int it = first; it < args.tokens * blocks; it += stride) {
     const int t = it / blocks, col = (it - t * blocks) * 32 * CPL + lane * CPL;
-    const int nb = (it - t * blocks) * 32 * CPL / 256;
-    // Lane j: row, gate and split shares of the token's j-th expert.
-    int row = 0, base = 0, g0 = 0, g1 = 0;
-    float gate = 0.f;
-    if (lane < topk) {
-      const int as = t * topk + lane;
-      row = args.row_of[as];
-      gate = args.gates[as];
-      const int a = args.act_of[as];
-      base = row - plan.act_off[a];
-      const int u = (nb * plan.active + a) * plan.steps2;
-      g0 = md_share_of(u, plan.units2, plan.shares2) + 1;
-      g1 = md_share_of(u + plan.steps2 - 1, plan.units2, plan.shares2);
+    MdSlot slot;
+    slot.load(args, plan, t, (it - t * blocks) * 32 * CPL / 256, lane);
+    if (!waited) {
+      const bool ok = lane != 0 || md_wait_counter(args.header + kMdDone2,
+                                                   4u * static_cast<uint32_t>(plan.units2), abort_flag, 40);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      __threadfence();
+      waited = true;
     }
     const bool in = col < K;
     const int c = col & 255;
     Vec v[kMdMaxTopk];
 #pragma unroll
     for (int j = 0; j < kMdMaxTopk; ++j) {
-      const int r = __shfl_sync(0xffffffffu, row, j);
+      const int r = __shfl_sync(0xffffffffu, slot.row, j);
       v[j].zero();
       if (j < topk && in) v[j].load(args.y + static_cast<size_t>(r) * K + col);
     }
 #pragma unroll
     for (int j = 0; j < kMdMaxTopk; ++j) {
       if (j >= topk) break;
-      const int b = __shfl_sync(0xffffffffu, base, j);
-      const int s0 = __shfl_sync(0xffffffffu, g0, j), s1 = __shfl_sync(0xffffffffu, g1, j);
+      const int b = __shfl_sync(0xffffffffu, slot.base, j);
+      const int s0 = __shfl_sync(0xffffffffu, slot.g0, j), s1 = __shfl_sync(0xffffffffu, slot.g1, j);
       for (int s = s0; s <= s1; s += 4) {
         Vec w[4];
 #pragma unroll
@@ -391,11 +416,12 @@ __device__ __forceinline__ void md_combine(const MoeDecodeArgs& args, const MdPl
     sum.zero();
 #pragma unroll
     for (int j = 0; j < kMdMaxTopk; ++j) {
-      const float g = __shfl_sync(0xffffffffu, gate, j);
+      const float g = __shfl_sync(0xffffffffu, slot.gate, j);
       if (j < topk) sum.fma(g, v[j]);
     }
     if (in) sum.template store<T>(static_cast<T*>(args.out) + static_cast<size_t>(t) * K + col);
   }
+  return true;
 }
 
 template <typename T>
@@ -480,7 +506,9 @@ __global__ void __launch_bounds__(kMdThreads, 1)
   plan.act_off = s_act_off;
   plan.row_token = s_row_token;
   const int shares = args.shares;
-  plan.shares1 = max(1, min(shares, plan.units1 / kMdMinSteps));
+  const int tiles = plan.active * plan.tiles1;
+  plan.whole1 = (tiles + shares - 1) / shares * plan.steps1 <= plan.units1 / shares + kMdSplitSteps;
+  plan.shares1 = plan.whole1 ? min(shares, tiles) : max(1, min(shares, plan.units1 / kMdMinSteps));
   plan.shares2 = max(1, min(shares, plan.units2 / kMdMinSteps));
   plan.claims = plan.shares1 + plan.shares2 + shares;
 
@@ -654,17 +682,12 @@ __global__ void __launch_bounds__(kMdThreads, 1)
       int share;
       const int ph = md_phase(plan, claim, &share);
       if (ph == 2) {
-        ok = lane != 0 || md_wait_counter(args.header + kMdDone2,
-                                          4u * static_cast<uint32_t>(plan.units2), abort_flag, 40);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        __threadfence();
-        // One warp per item of one token and 32 CPL columns; eight columns a
-        // lane where that keeps every warp of the grid at work, two where not.
-        const int blocks = (K + 255) / 256;
-        if (args.tokens * blocks >= 4 * shares)
-          md_combine<T, 8>(args, plan, 4 * share + q, 4 * shares, lane);
-        else
-          md_combine<T, 2>(args, plan, 4 * share + q, 4 * shares, lane);
+        // One warp per item of one token and 32 CPL columns: two columns a lane
+        // where every item has a warp of the grid to itself, else eight.
+        ok = args.tokens * ((K + 63) / 64) > 4 * shares
+                 ? md_combine<T, 8>(args, plan, 4 * share + q, 4 * shares, lane, abort_flag)
+                 : md_combine<T, 2>(args, plan, 4 * share + q, 4 * shares, lane, abort_flag);
+        if (!ok) break;
         if (lane == 0) mbar_arrive(&qempty[qslot]);
         continue;
       }

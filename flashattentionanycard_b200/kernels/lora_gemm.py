@@ -104,34 +104,25 @@ def launch(x, w, bank, ids, out, workspace=None):
     n = w.shape[1]
     if w.shape[0] != k or out.shape != (m, n):
         raise ValueError(f"shape mismatch: x {tuple(x.shape)}, w {tuple(w.shape)}, out {tuple(out.shape)}")
-    if (k, n) != (bank.k, bank.n):
+    if k != bank.k or n != bank.n:
         raise ValueError(f"the bank's adapters are for a [{bank.k}, {bank.n}] projection, not [{k}, {n}]")
     if ids.dtype != torch.int32 or ids.shape != (m,) or not ids.is_contiguous():
         raise ValueError(f"ids must be a contiguous int32 tensor of {m} elements")
-    if not (x.dtype == w.dtype == out.dtype == bank.dtype):
+    dtype = x.dtype
+    if not (dtype == w.dtype == out.dtype == bank.dtype):
         raise ValueError("x, w, out and the bank must share one dtype")
     if not (x.is_contiguous() and w.is_contiguous() and out.is_contiguous()):
         raise ValueError("x, w and out must be contiguous row-major tensors")
-    device = x.device
-    if not (x.is_cuda and w.device == device and out.device == device and ids.device == device
-            and bank.device == device):
+    index = x.get_device()
+    if index < 0 or not (w.get_device() == out.get_device() == ids.get_device() == bank.a.get_device() == index):
         raise ValueError("all tensors and the bank must be on one CUDA device")
     lib = _native.load()
-    with _native.on_device(device):
-        need = lib.bokt_lora_gemm_workspace_bytes(m, n, k, bank.slots, bank.rank)
-        if need < 0:
-            raise RuntimeError(f"bokt_lora_gemm: {lib.bokt_last_error().decode()}")
-        if workspace is None:
-            workspace = torch.empty(need, device=device, dtype=torch.uint8)
-        elif workspace.device != device or not workspace.is_contiguous() \
-                or workspace.numel() * workspace.element_size() < need:
-            raise ValueError(f"workspace must be a contiguous tensor of {need} bytes on {device}")
-        _native.check(
-            lib.bokt_lora_gemm(
-                x.data_ptr(), w.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
-                bank.ranks.data_ptr(), ids.data_ptr(), out.data_ptr(), m, n, k, bank.slots, bank.rank,
-                _native.dtype_code(x.dtype), workspace.data_ptr(),
-                workspace.numel() * workspace.element_size(), _native.current_stream(device)),
-            "bokt_lora_gemm",
-        )
+    with _native.on_device(index):
+        scratch, nbytes = _native.workspace("bokt_lora_gemm_workspace_bytes", (m, n, k, bank.slots, bank.rank),
+                                            index, workspace)
+        rc = lib.bokt_lora_gemm(
+            x.data_ptr(), w.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
+            bank.ranks.data_ptr(), ids.data_ptr(), out.data_ptr(), m, n, k, bank.slots, bank.rank,
+            _native.dtype_code(dtype), scratch.data_ptr(), nbytes, _native.current_stream(index))
+    _native.check(rc, "bokt_lora_gemm")
     return out

@@ -38,16 +38,17 @@ def launch(x, logits, w_gate_up, w_down, out, topk, renormalize=True, workspace=
     torch's allocator."""
     import torch
 
-    if x.dim() != 2 or w_gate_up.dim() != 3 or w_down.dim() != 3 or logits.dim() != 2:
+    xs, gs, ds, ls = x.shape, w_gate_up.shape, w_down.shape, logits.shape
+    if len(xs) != 2 or len(gs) != 3 or len(ds) != 3 or len(ls) != 2:
         raise ValueError("x and logits must have two dimensions, the weights three")
-    t, k = x.shape
-    e, inner = w_gate_up.shape[0], w_down.shape[1]
+    t, k = xs
+    e, inner, _ = ds
     topk = int(topk)
-    if w_gate_up.shape != (e, k, 2 * inner) or w_down.shape != (e, inner, k):
-        raise ValueError(f"shape mismatch: x {tuple(x.shape)}, w_gate_up {tuple(w_gate_up.shape)} "
-                         f"(expected [E, K, 2 I]), w_down {tuple(w_down.shape)} (expected [E, I, K])")
-    if logits.shape != (t, e) or out.shape != (t, k):
-        raise ValueError(f"shape mismatch: logits {tuple(logits.shape)}, out {tuple(out.shape)}")
+    if gs != (e, k, 2 * inner) or ds != (e, inner, k):
+        raise ValueError(f"shape mismatch: x {tuple(xs)}, w_gate_up {tuple(gs)} "
+                         f"(expected [E, K, 2 I]), w_down {tuple(ds)} (expected [E, I, K])")
+    if ls != (t, e) or out.shape != xs:
+        raise ValueError(f"shape mismatch: logits {tuple(ls)}, out {tuple(out.shape)}")
     if not 1 <= topk <= min(e, MAX_TOPK):
         raise ValueError(f"topk must be in [1, {min(e, MAX_TOPK)}], got {topk}")
     if t > MAX_TOKENS or e > MAX_EXPERTS:
@@ -57,33 +58,22 @@ def launch(x, logits, w_gate_up, w_down, out, topk, renormalize=True, workspace=
         raise ValueError(f"K and I must be multiples of 8 (got {k} and {inner})")
     if not (x.dtype == w_gate_up.dtype == w_down.dtype == out.dtype):
         raise ValueError("x, the weights and out must share one dtype")
-    if logits.dtype == torch.float32:
-        logits_dtype = 2
-    else:
-        logits_dtype = _native.dtype_code(logits.dtype)
+    logits_dtype = 2 if logits.dtype == torch.float32 else _native.dtype_code(logits.dtype)
     dtype = _native.dtype_code(x.dtype)
-    tensors = (x, logits, w_gate_up, w_down, out)
-    if not all(v.is_contiguous() for v in tensors):
+    if not (x.is_contiguous() and logits.is_contiguous() and w_gate_up.is_contiguous()
+            and w_down.is_contiguous() and out.is_contiguous()):
         raise ValueError("x, logits, the weights and out must be contiguous")
-    device = x.device
-    if not (x.is_cuda and all(v.device == device for v in tensors)):
+    index = x.get_device()
+    if index < 0 or not (logits.get_device() == w_gate_up.get_device() == w_down.get_device()
+                         == out.get_device() == index):
         raise ValueError("all tensors must be on one CUDA device")
     lib = _native.load()
-    with _native.on_device(device):
-        need = lib.bokt_moe_decode_workspace_bytes(t, e, k, inner, topk)
-        if need < 0:
-            raise RuntimeError(f"bokt_moe_decode: {lib.bokt_last_error().decode()}")
-        if workspace is None:
-            workspace = torch.empty(need, device=device, dtype=torch.uint8)
-        elif workspace.device != device or not workspace.is_contiguous() \
-                or workspace.numel() * workspace.element_size() < need:
-            raise ValueError(f"workspace must be a contiguous tensor of {need} bytes on {device}")
-        _native.check(
-            lib.bokt_moe_decode(
-                x.data_ptr(), logits.data_ptr(), logits_dtype, w_gate_up.data_ptr(), w_down.data_ptr(),
-                out.data_ptr(), t, e, k, inner, topk, 1 if renormalize else 0, dtype,
-                workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                _native.current_stream(device)),
-            "bokt_moe_decode",
-        )
+    with _native.on_device(index):
+        scratch, nbytes = _native.workspace("bokt_moe_decode_workspace_bytes", (t, e, k, inner, topk), index,
+                                            workspace)
+        rc = lib.bokt_moe_decode(
+            x.data_ptr(), logits.data_ptr(), logits_dtype, w_gate_up.data_ptr(), w_down.data_ptr(),
+            out.data_ptr(), t, e, k, inner, topk, 1 if renormalize else 0, dtype, scratch.data_ptr(), nbytes,
+            _native.current_stream(index))
+    _native.check(rc, "bokt_moe_decode")
     return out
