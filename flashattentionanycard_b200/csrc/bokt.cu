@@ -1870,7 +1870,7 @@ constexpr int kLoraShrinkSmem = 20 * 1024;
 struct LoraPlan {
   bool stream;
   int tile_rows, tiles, smax, gmax, cluster, stages;
-  int shrink_cluster, shrink_mt, walkers;
+  int shrink_cluster, walkers;
   int64_t count, list, h, total;
 };
 
@@ -1944,14 +1944,11 @@ int lora_plan(int M, int N, int K, int slots, int rank, const DeviceInfo& dev, L
   }
   p->smax = slots < p->tile_rows ? slots : p->tile_rows;
   if (M < p->smax && M > 0) p->smax = M;
-  // The shrink: row tiles of many tokens walk an adapter's tokens 32 at a time
-  // over clusters of eight CTAs; few tokens split K as far as there are SMs.
-  p->shrink_mt = p->stream ? 1 : 2;
+  // The shrink of few tokens splits K as far as there are SMs.
   p->shrink_cluster = 8;
-  if (p->stream)
-    while (p->shrink_cluster > 1 && ((long long)p->tiles * p->smax * p->shrink_cluster > dev.sm_count ||
-                                     K < p->shrink_cluster * 256))
-      p->shrink_cluster /= 2;
+  while (p->shrink_cluster > 1 && ((long long)p->tiles * p->smax * p->shrink_cluster > dev.sm_count ||
+                                   K < p->shrink_cluster * 256))
+    p->shrink_cluster /= 2;
   const long long want = dev.sm_count / ((long long)p->shrink_cluster * (p->tiles ? p->tiles : 1));
   p->walkers = int(want < 1 ? 1 : (want < p->smax ? want : p->smax));
   p->gmax = (p->smax * rank + 63) / 64;
@@ -1979,18 +1976,18 @@ cudaError_t launch_cluster(const void* fn, int grid, int threads, int smem, int 
   return cudaLaunchKernelExC(&lc, fn, kargs);
 }
 
-template <typename T, int MT>
+template <typename T>
 const void* lora_shrink_ptr(int rank, int* smem) {
   if (rank == 16) {
-    *smem = bokt::lora_shrink_smem_bytes<MT, 2>();
-    return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, MT, 2>);
+    *smem = bokt::lora_shrink_smem_bytes<2>();
+    return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, 2>);
   }
   if (rank == 32) {
-    *smem = bokt::lora_shrink_smem_bytes<MT, 4>();
-    return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, MT, 4>);
+    *smem = bokt::lora_shrink_smem_bytes<4>();
+    return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, 4>);
   }
-  *smem = bokt::lora_shrink_smem_bytes<MT, 8>();
-  return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, MT, 8>);
+  *smem = bokt::lora_shrink_smem_bytes<8>();
+  return reinterpret_cast<const void*>(&bokt::lora_shrink_kernel<T, 8>);
 }
 
 }  // namespace
@@ -2068,25 +2065,35 @@ int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void*
     const uint32_t b[3] = {64, rs, 1};
     if ((rc = encode_map(&mb, lora_b, 3, d, st, b, fp16))) return rc;
   }
-  {
-    const bool bf = dtype == BOKT_BF16;
+  cudaError_t e;
+  if (p.stream) {
     int smem = 0;
-    const void* fn = p.shrink_mt == 2 ? (bf ? lora_shrink_ptr<__nv_bfloat16, 2>(rank, &smem)
-                                            : lora_shrink_ptr<__half, 2>(rank, &smem))
-                                      : (bf ? lora_shrink_ptr<__nv_bfloat16, 1>(rank, &smem)
-                                            : lora_shrink_ptr<__half, 1>(rank, &smem));
+    const void* fn = fp16 ? lora_shrink_ptr<__half>(rank, &smem) : lora_shrink_ptr<__nv_bfloat16>(rank, &smem);
     if ((rc = ensure_smem(fn, smem)) || (rc = ensure_carveout(fn))) return rc;
-    const int clusters = p.tiles * p.walkers;
     a.cluster = p.shrink_cluster;
     a.walkers = p.walkers;
     void* kargs[] = {&x, &lora_a, &a};
-    const int threads = 32 * (p.shrink_mt == 2 ? bokt::lora_shrink_warps<2>() : bokt::lora_shrink_warps<1>());
-    cudaError_t e = launch_cluster(fn, clusters * a.cluster, threads, smem, a.cluster, s, kargs);
-    if (e != cudaSuccess) return cuda_fail(e, "lora_shrink launch");
+    e = launch_cluster(fn, p.tiles * p.walkers * a.cluster, bokt::kLoraThreads, smem, a.cluster, s, kargs);
+  } else {
+    CUtensorMap ma;
+    const uint64_t d[2] = {uint64_t(K), uint64_t(slots) * rank};
+    const uint64_t st[1] = {uint64_t(K) * 2};
+    const uint32_t b[2] = {64, rs};
+    if ((rc = encode_map(&ma, lora_a, 2, d, st, b, fp16))) return rc;
+    a.idesc = bokt::make_idesc_f16_kk(uint32_t(dtype), 0);
+    a.stages = 5;
+    const int smem = bokt::lora_shrink_tc_smem_bytes(a.stages);
+    const void* fn = fp16 ? reinterpret_cast<const void*>(&bokt::lora_shrink_tc_kernel<__half>)
+                          : reinterpret_cast<const void*>(&bokt::lora_shrink_tc_kernel<__nv_bfloat16>);
+    if ((rc = ensure_smem(fn, smem))) return rc;
+    const int clusters = (M + bokt::kLoraShrinkRows - 1) / bokt::kLoraShrinkRows;
+    void* kargs[] = {&mx, &ma, &a};
+    e = launch_cluster(fn, clusters * bokt::kLoraShrinkSplit, bokt::kLoraThreads, smem,
+                       bokt::kLoraShrinkSplit, s, kargs);
   }
+  if (e != cudaSuccess) return cuda_fail(e, "lora_shrink launch");
   a.cluster = p.cluster;
   a.stages = p.stages;
-  cudaError_t e;
   if (p.stream) {
     a.idesc = bokt::make_idesc_f16_swapped(uint32_t(dtype), uint32_t(p.tile_rows));
     const void* fn = fp16 ? reinterpret_cast<const void*>(&bokt::lora_stream_kernel<__half>)

@@ -266,6 +266,11 @@ __host__ __device__ constexpr uint32_t make_idesc_f16_swapped(uint32_t ab_format
          ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
+// The same with A and B both K-major (tokens against rows of a [rank, K] factor).
+__host__ __device__ constexpr uint32_t make_idesc_f16_kk(uint32_t ab_format, uint32_t n) {
+  return (1u << 4) | (ab_format << 7) | (ab_format << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
 // ---------------------------------------------------------------------------
 // Element conversion helpers.
 // ---------------------------------------------------------------------------

@@ -10,11 +10,13 @@
 // tensor-core operand).  The zeros of H_j meet B of other tokens' adapters, so
 // B must be finite; the bank refuses adapters that are not.
 //
-//   lora_shrink_kernel  H (and each row tile's list of adapters).  HBM / latency
-//       bound; a cluster per (row tile, adapter), its tokens gathered 16 or 32
+//   lora_shrink_kernel  H (and each row tile's list of adapters) for few tokens.
+//       Latency bound; a cluster per (row tile, adapter), its tokens gathered 16
 //       at a time, K split over warps and CTAs; warp-level mma.sync on fragments
 //       loaded straight from global memory (few flops: a 128-row tcgen05 tile
 //       would idle on an adapter's handful of tokens).
+//   lora_shrink_tc_kernel  the same for many tokens: bound by reading x; 128
+//       tokens a cluster of four CTAs that split K, TMA ring and tcgen05.
 //   lora_stream_kernel  few tokens (row tiles of up to 128): bound by reading W.
 //       W tiles are the 128-row operand and the tokens the narrow one; a cluster
 //       of C CTAs splits K and reduces through distributed shared memory.
@@ -90,31 +92,24 @@ __device__ __forceinline__ void st_cluster_u32x4(uint32_t addr, uint32_t a, uint
                : "memory");
 }
 
-// Row tiles of many tokens (MT = 2) have few clusters to hide latency with:
-// twice the warps.
-template <int MT>
-__host__ __device__ constexpr int lora_shrink_warps() {
-  return MT == 1 ? 8 : 16;
-}
-template <int MT, int RN>
+template <int RN>
 __host__ __device__ constexpr int lora_shrink_smem_bytes() {
-  return (lora_shrink_warps<MT>() + 1) * 16 * MT * RN * 8 * 4;  // a partial per warp, their sum
+  return (8 + 1) * 16 * RN * 8 * 4;  // a partial per warp, their sum
 }
 
 // Cluster (row tile, w) takes the tile's list entries w, w + walkers, ...: for
 // adapter a_j all rows of H_j, the products of its own tokens and zeros for the
-// others.  The tokens are walked in groups of 16 MT; kc CTAs of the cluster
+// others.  The tokens are walked in groups of 16; kc CTAs of the cluster
 // share a group and split its K (all of them for one group, one each for as
 // many groups as CTAs).  A lane's 16-byte loads hold 8 neighbouring k-values of
 // one row; two mma.sync take them as their k-fragments (the same k-order on
 // both sides, so the dot products are whole).  Partial sums meet over the warps
 // in shared memory and over the CTAs through distributed shared memory, in
 // order.
-template <typename T, int MT, int RN>
-__global__ void __launch_bounds__(32 * lora_shrink_warps<MT>(), MT == 1 ? 2 : 1)
+template <typename T, int RN>
+__global__ void __launch_bounds__(kLoraThreads, 2)
     lora_shrink_kernel(const T* x, const T* lora_a, const LoraArgs args) {
-  constexpr int kTok = 16 * MT, kCols = RN * 8;
-  constexpr int NW = lora_shrink_warps<MT>(), kThreads = 32 * NW;
+  constexpr int kTok = 16, kCols = RN * 8, NW = 8, kThreads = kLoraThreads;
   constexpr int kVotes = kLoraMaxSlots / kThreads;  // slots per lane
   extern __shared__ float sm[];
   float* part = sm;                      // [NW][kTok][kCols]
@@ -203,42 +198,36 @@ __global__ void __launch_bounds__(32 * lora_shrink_warps<MT>(), MT == 1 ? 2 : 1)
       const T* ar = lora_a + (static_cast<size_t>(id) * args.rank + r0 + g) * args.K + q * 8;
       for (int it = 0; it * stride < groups; ++it) {
         const int t0 = (it * stride + rank / kc) * kTok;
-        const T* xr[2 * MT];  // rows g, g + 8, ... of the group (past its end: dropped below)
+        const T* xr[2];  // rows g, g + 8, ... of the group (past its end: dropped below)
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i)
+        for (int i = 0; i < 2; ++i)
           xr[i] = xt + static_cast<size_t>(s_rows[t0 + 8 * i + g < tokens ? t0 + 8 * i + g : 0]) * args.K + q * 8;
-        float acc[MT][RN][4] = {};
+        float acc[RN][4] = {};
         if (t0 < tokens) {
 #pragma unroll 2
           for (int k = (sub * NW + warp) * 32; k < args.K; k += kc * NW * 32) {
             const bool in = k + q * 8 < args.K;  // K is a multiple of 8
-            uint4 xa[2 * MT], bv[RN];
+            uint4 xa[2], bv[RN];
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i)
+            for (int i = 0; i < 2; ++i)
               xa[i] = in ? *reinterpret_cast<const uint4*>(xr[i] + k) : make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int n = 0; n < RN; ++n)
               bv[n] = in ? *reinterpret_cast<const uint4*>(ar + static_cast<size_t>(n) * 8 * args.K + k)
                          : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-              for (int n = 0; n < RN; ++n) {
-                mma_16816<T>(acc[m][n], xa[2 * m].x, xa[2 * m + 1].x, xa[2 * m].y, xa[2 * m + 1].y,
-                             bv[n].x, bv[n].y);
-                mma_16816<T>(acc[m][n], xa[2 * m].z, xa[2 * m + 1].z, xa[2 * m].w, xa[2 * m + 1].w,
-                             bv[n].z, bv[n].w);
-              }
+            for (int n = 0; n < RN; ++n) {
+              mma_16816<T>(acc[n], xa[0].x, xa[1].x, xa[0].y, xa[1].y, bv[n].x, bv[n].y);
+              mma_16816<T>(acc[n], xa[0].z, xa[1].z, xa[0].w, xa[1].w, bv[n].z, bv[n].w);
+            }
           }
         }
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int n = 0; n < RN; ++n)
-              *reinterpret_cast<float2*>(part + (warp * kTok + 16 * m + 8 * half + g) * kCols + n * 8 + 2 * q) =
-                  make_float2(acc[m][n][2 * half], acc[m][n][2 * half + 1]);
+          for (int n = 0; n < RN; ++n)
+            *reinterpret_cast<float2*>(part + (warp * kTok + 8 * half + g) * kCols + n * 8 + 2 * q) =
+                make_float2(acc[n][2 * half], acc[n][2 * half + 1]);
         __syncthreads();
         for (int i = tid; i < kTok * kCols; i += kThreads) {
           const int row = i / kCols, c = i % kCols;
@@ -292,6 +281,245 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+}
+
+constexpr int kLoraShrinkRows = 128, kLoraShrinkSplit = 4;  // tokens and CTAs of a cluster
+constexpr int kLoraShrinkCols = 128;                        // accumulator columns of a pass
+constexpr int kLoraShrinkStage = (kLoraShrinkRows + kLoraShrinkCols) * 128;
+constexpr int kLoraShrinkRecv = kLoraShrinkSplit * 32 * 64 * 4;
+
+__host__ __device__ inline int lora_shrink_tc_smem_bytes(int stages) {
+  return 1024 + stages * kLoraShrinkStage + kLoraShrinkRecv + (2 * stages + 2) * 8 + 16;
+}
+
+// H and the lists for row tiles of kLoraPairRows, many tokens.  A cluster takes
+// 128 tokens; CTA r runs a quarter of K: x as the 128-row operand, the A rows of
+// the adapters that these tokens use as the narrow one, 128 columns (128 / R
+// adapters) a pass.  A token keeps the columns of its own adapter; CTA r sums
+// and writes those of tokens [32 r, +32) after the quarters have met in its
+// shared memory, in rank order.
+template <typename T>
+__global__ void __launch_bounds__(kLoraThreads, 1)
+    lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tm_x,
+                          const __grid_constant__ CUtensorMap tm_a, const LoraArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int stages = args.stages;
+  float* recv = reinterpret_cast<float*>(smem + stages * kLoraShrinkStage);  // [4][32][rs]
+  uint64_t* full = reinterpret_cast<uint64_t*>(recv + kLoraShrinkRecv / 4);
+  uint64_t* empty = full + stages;
+  uint64_t* tfull = empty + stages;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tfull + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  __shared__ int s_flag[kLoraMaxSlots];  // 1 used by the row tile, 3 also by these tokens; then the place
+  __shared__ int s_place[kLoraPairRows];  // of these tokens' adapters: place in the row tile's list
+  __shared__ int s_slot[kLoraPairRows];   // and slot
+  __shared__ int s_id[kLoraShrinkRows], s_warp[8], s_mine[8];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int t0 = static_cast<int>(blockIdx.x) / kLoraShrinkSplit * kLoraShrinkRows;
+  const int mt = t0 / kLoraPairRows, m0 = mt * kLoraPairRows;
+  const int R = args.rank, rs = min(R, 64);
+  const int nkb = (args.K + 63) / 64;
+  const int kb0 = rank * nkb / kLoraShrinkSplit, kb1 = (rank + 1) * nkb / kLoraShrinkSplit;
+
+  if (tid == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(tfull, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_a);
+  }
+  if (warp == 3) {
+    tmem_alloc(tmem_holder, kLoraShrinkCols);
+    tmem_relinquish();
+  }
+  for (int i = tid; i < args.slots; i += kLoraThreads) s_flag[i] = 0;
+  cluster_sync();  // every CTA runs before another writes its shared memory
+  pdl_wait();
+  pdl_allow_next();
+  // Adapters of the row tile (256 rows, one per thread) and of these 128 tokens.
+  int my_id = -1;
+  const bool here = m0 + tid >= t0 && m0 + tid < t0 + kLoraShrinkRows;
+  if (m0 + tid < args.M) {
+    const int id = args.ids[m0 + tid];
+    if (id >= 0 && id < args.slots && args.ranks[id] > 0) {
+      my_id = id;
+      atomicOr(&s_flag[id], here ? 3 : 1);
+    } else if (id != -1 && here && rank == 0) {
+      report_status(kStatusBadAdapter, m0 + tid);
+    }
+  }
+  if (here) s_id[m0 + tid - t0] = my_id;
+  __syncthreads();
+  int place[4], mine[4], used = 0, own = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int slot = warp * 128 + i * 32 + lane;
+    const int f = slot < args.slots ? s_flag[slot] : 0;
+    const unsigned b = __ballot_sync(0xffffffffu, f != 0), c = __ballot_sync(0xffffffffu, f == 3);
+    const unsigned below = (1u << lane) - 1u;
+    place[i] = f != 0 ? used + __popc(b & below) : -1;
+    mine[i] = f == 3 ? own + __popc(c & below) : -1;
+    used += __popc(b);
+    own += __popc(c);
+  }
+  if (lane == 0) {
+    s_warp[warp] = used;
+    s_mine[warp] = own;
+  }
+  __syncthreads();
+  int before = 0, total = 0, before_own = 0, adapters = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    before += w < warp ? s_warp[w] : 0;
+    before_own += w < warp ? s_mine[w] : 0;
+    total += s_warp[w];
+    adapters += s_mine[w];
+  }
+  const bool writes_list = rank == 0 && t0 == m0;
+  if (writes_list && tid == 0) args.count[mt] = total;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int slot = warp * 128 + i * 32 + lane;
+    if (place[i] < 0) continue;
+    s_flag[slot] = before + place[i];
+    if (writes_list) args.list[mt * args.smax + before + place[i]] = slot;
+    if (mine[i] >= 0) {
+      s_place[before_own + mine[i]] = before + place[i];
+      s_slot[before_own + mine[i]] = slot;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+
+  T* h = static_cast<T*>(args.h) + static_cast<size_t>(mt) * args.gmax * kLoraPairRows * 64;
+  const size_t group = static_cast<size_t>(kLoraPairRows) * 64;
+  const int per_pass = kLoraShrinkCols / R;
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int p0 = 0, pass = 0; p0 < adapters; p0 += per_pass, ++pass) {
+    const int na = min(per_pass, adapters - p0);
+    if (warp == 0) {
+      if (elect_one()) {
+        for (int kb = kb0; ok && kb < kb1; ++kb) {
+          if (!(ok = mbar_wait(&empty[stage], phase ^ 1u, abort_flag, 71))) break;
+          uint8_t* b = smem + stage * kLoraShrinkStage;
+          mbar_arrive_expect_tx(&full[stage], kLoraShrinkRows * 128 + na * R * 128);
+          tma_load_2d(b, &tm_x, &full[stage], kb * 64, t0);
+          b += kLoraShrinkRows * 128;
+          for (int c = 0; c < na * R; c += rs)
+            tma_load_2d(b + c * 128, &tm_a, &full[stage], kb * 64, s_slot[p0 + c / R] * R + c % R);
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (elect_one()) {
+        const uint32_t idesc = args.idesc | (static_cast<uint32_t>(na * R >> 3) << 17);
+        for (int kb = kb0; ok && kb < kb1; ++kb) {
+          if (!(ok = mbar_wait(&full[stage], phase, abort_flag, 72))) break;
+          tc_fence_after();
+          const uint32_t a = smem_addr(smem + stage * kLoraShrinkStage);
+          const uint32_t b = a + kLoraShrinkRows * 128;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16_ss(tmem_base, smem_desc_sw128(a + k * 32, 16, 1024),
+                        smem_desc_sw128(b + k * 32, 16, 1024), idesc, kb != kb0 || k != 0 ? 1u : 0u);
+          umma_commit(&empty[stage]);
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) umma_commit(tfull);
+      }
+    }
+    __syncwarp();
+    const bool done = mbar_wait(tfull, pass & 1, abort_flag, 73);
+    for (int r0 = 0; r0 < R; r0 += 64) {
+      if (warp >= 4 && __all_sync(0xffffffffu, done)) {
+        // Warp q holds tokens [32 q, +32), a lane each; their sums go to CTA q.
+        const int q = warp & 3;
+        tc_fence_after();
+        const int id = s_id[q * 32 + lane];
+        const uint32_t at = map_shared(smem_addr(recv + (rank * 32 + lane) * rs), q);
+        for (int e = 0; e < na; ++e) {
+          const bool is_mine = s_slot[p0 + e] == id;
+          if (!__any_sync(0xffffffffu, is_mine)) continue;
+          for (int c = 0; c < rs; c += 16) {
+            uint32_t v[16];
+            tmem_ld_32x32b_x16(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + e * R + r0 + c, v);
+            tmem_ld_wait();
+            if (is_mine) {
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                // A CTA without k-steps has accumulated nothing.
+                const bool some = kb1 > kb0;
+                st_cluster_u32x4(at + (c + j) * 4, some ? v[j] : 0u, some ? v[j + 1] : 0u,
+                                 some ? v[j + 2] : 0u, some ? v[j + 3] : 0u);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+      }
+      cluster_sync();
+      for (int i = tid; i < 32 * rs / 2; i += kLoraThreads) {
+        const int tok = i / (rs / 2), c = i % (rs / 2) * 2;
+        const int id = s_id[rank * 32 + tok];
+        if (id < 0) continue;
+        const int j = s_flag[id];
+        if (j < s_place[p0] || j > s_place[p0 + na - 1]) continue;  // another pass's adapter
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int s = 0; s < kLoraShrinkSplit; ++s) {
+          const float2 v = *reinterpret_cast<const float2*>(recv + (s * 32 + tok) * rs + c);
+          sum.x += v.x;
+          sum.y += v.y;
+        }
+        // Past the adapter's own rank H is 0 whatever x holds.
+        const int own_rank = args.ranks[id];
+        const float scale = args.scales[id];
+        sum.x = r0 + c < own_rank ? sum.x * scale : 0.f;
+        sum.y = r0 + c + 1 < own_rank ? sum.y * scale : 0.f;
+        const int col = j * R + r0 + c;
+        *reinterpret_cast<uint32_t*>(h + col / 64 * group + (t0 - m0 + rank * 32 + tok) * 64 + col % 64) =
+            Pack2<T>::pack(sum.x, sum.y);
+      }
+      cluster_sync();  // read before the next columns overwrite them, or the CTA leaves
+    }
+  }
+  // Zeros where a token meets another adapter of its row tile.
+  const int vecs = R / 8;
+  for (int i = tid; i < 32 * total * vecs; i += kLoraThreads) {
+    const int v = i % vecs, e = i / vecs % total, tok = rank * 32 + i / (vecs * total);
+    if (t0 + tok >= args.M || (s_id[tok] >= 0 && s_flag[s_id[tok]] == e)) continue;
+    const int col = e * R + v * 8;
+    *reinterpret_cast<uint4*>(h + col / 64 * group + (t0 - m0 + tok) * 64 + col % 64) = make_uint4(0, 0, 0, 0);
+  }
+  if (*abort_flag && tid == 0) {
+    // After a given-up wait: let copies in flight land before the CTA leaves.
+    const uint64_t start = globaltimer_ns();
+    while (globaltimer_ns() - start < 2000000ull) {
+    }
+  }
+  __syncthreads();
+  if (warp == 3) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kLoraShrinkCols);
+  }
 }
 
 __host__ __device__ inline int lora_stream_smem_bytes(int nt, int stages) {
