@@ -1502,7 +1502,7 @@ extern "C" int bokt_moe_route_noalloc(const int32_t* expert_ids, int A, int E, i
 namespace {
 
 // Blocks per SM of the persistent backward kernel (its partial rows are sized by this).
-constexpr int kQkGradBlocksPerSm = 4;
+constexpr int kQkGradBlocksPerSm = 2;
 
 bool qk_strides_vec(const bokt::QkSide& s) {
   return ((s.x_row | s.x_head | s.g_row | s.g_head | s.out_row | s.out_head) & 7) == 0 &&
@@ -1535,8 +1535,10 @@ cudaError_t launch_qk_vec(bokt::QkArgs a, int sm_count, int* blocks, cudaStream_
     if (grid > (long long)kQkGradBlocksPerSm * sm_count)
       grid = (long long)kQkGradBlocksPerSm * sm_count;
     *blocks = int(grid);
-    return launch(bokt::qk_norm_rope_grad_kernel<T, L, PAIRS, R>, dim3(unsigned(grid)),
-                  dim3(bokt::kQkThreads), 0, s, a);
+    auto* kernel = bokt::qk_norm_rope_grad_kernel<T, L, PAIRS, R>;
+    const int smem = bokt::qk_grad_smem_bytes<L, R>();
+    if (ensure_smem(reinterpret_cast<const void*>(kernel), smem)) return cudaErrorInvalidValue;
+    return launch(kernel, dim3(unsigned(grid)), dim3(bokt::kQkThreads), smem, s, a);
   } else {
     *blocks = 0;
     return launch(bokt::qk_norm_rope_kernel<T, L, PAIRS, R>,

@@ -221,14 +221,47 @@ __global__ void __launch_bounds__(kQkThreads, 4) qk_norm_rope_kernel(const QkArg
   }
 }
 
-// Backward: persistent warps walk the query units, then the key units; the
-// weight gradient of a side stays in 8 registers per lane until its last unit,
-// is summed over the block's rows in shared memory and leaves as one partial
-// row per block, which qk_norm_rope_dweight_kernel adds in block order.
+// 16 bytes to shared memory without passing through registers; zeros where the
+// lane has nothing to read.
+__device__ __forceinline__ void qk_copy_async(uint4* dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src),
+               "r"(in ? 16 : 0)
+               : "memory");
+}
+
+// Rows of one warp's walk: batches of R heads per lane group, unit after unit.
+struct QkWalk {
+  int u, t, h0, hend;
+  __device__ __forceinline__ void enter(int unit, int chunks, int hpu, int heads, int sub) {
+    u = unit;
+    t = unit / chunks;
+    const int chunk = unit - t * chunks;
+    h0 = chunk * hpu + sub;
+    hend = min(heads, (chunk + 1) * hpu);
+  }
+};
+
+constexpr int kQkRing = 3;  // batches in flight or in use per warp
+
+// Shared memory of the backward kernel: a ring of R rows of x and of the
+// gradient per lane, and the block's sums.
+template <int L, int R>
+__host__ __device__ constexpr int qk_grad_smem_bytes() {
+  const int ring = kQkThreads * kQkRing * R * 2 * 16;
+  const int sums = kQkWarps * (32 / L) * (L * 8 + 1) * 4;
+  return ring > sums ? ring : sums;
+}
+
+// Backward: persistent warps walk the query units, then the key units.  The
+// next batches' rows arrive by cp.async while one is computed (each lane reads
+// back what it copied itself: no barrier); the weight gradient of a side stays
+// in 8 registers per lane until its last unit, is summed over the block's rows
+// in shared memory and leaves as one partial row per block, which
+// qk_norm_rope_dweight_kernel adds in block order.
 template <typename T, int L, bool PAIRS, int R>
 __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const QkArgs args) {
   constexpr int S = 32 / L;
-  __shared__ float sums[kQkWarps * S][L * 8 + 1];
+  extern __shared__ uint4 qk_ring[];
   pdl_allow_next();
   const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L, warp = threadIdx.x >> 5;
   const int i = l * 8;
@@ -237,6 +270,8 @@ __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const 
   const bool turns = i < args.rot;
   const int half = args.rot / 16;
   const int partner = PAIRS || !turns ? lane : (i < args.rot / 2 ? lane + half : lane - half);
+  uint4* ring = qk_ring + threadIdx.x;  // [slot][row][x, gradient][thread]
+  const int stride = gridDim.x * kQkWarps;
   pdl_wait();
 #pragma unroll 1
   for (int side = 0; side < 2; ++side) {
@@ -247,63 +282,88 @@ __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const 
     float w[8], dw[8] = {};
     qk_unpack<T>(active && units > 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(sd.w) + i)
                                      : make_uint4(0, 0, 0, 0), w);
-#pragma unroll 1
-    for (int u = blockIdx.x * kQkWarps + warp; u < units; u += gridDim.x * kQkWarps) {
-      const int t = u / chunks;
-      const int hend = min(sd.heads, (u - t * chunks + 1) * hpu);
-      const long long pos = qk_position(args, t);
-      if (pos < 0 || pos >= args.table_rows) {
-        if (lane == 0) report_status(kStatusBadPosition, t);
-        continue;
-      }
-      QkAngles ang;
-      if (turns) qk_load_angles<PAIRS>(args.cos_sin + pos * args.rot, args.rot, i, ang);
-      const T* x = static_cast<const T*>(sd.x) + t * sd.x_row + i;
-      const T* g = static_cast<const T*>(sd.g) + t * sd.g_row + i;
-      T* out = static_cast<T*>(sd.out) + t * sd.out_row + i;
-      for (int h0 = (u - t * chunks) * hpu + sub; h0 - sub < hend; h0 += S * R) {
-        uint4 xr[R], gr[R];
+    QkWalk in = {}, at = {};  // the batch to copy next, the batch to compute
+    in.u = at.u = blockIdx.x * kQkWarps + warp;
+    if (in.u < units) in.enter(in.u, chunks, hpu, sd.heads, sub);
+    int slot_in = 0, slot = 0;
+    auto copy = [&] {
+      if (in.u < units) {
+        const T* x = static_cast<const T*>(sd.x) + in.t * sd.x_row + i;
+        const T* g = static_cast<const T*>(sd.g) + in.t * sd.g_row + i;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const int h = h0 + r * S;
-          const bool in = active && h < hend;
-          xr[r] = in ? *reinterpret_cast<const uint4*>(x + h * sd.x_head) : make_uint4(0, 0, 0, 0);
-          gr[r] = in ? *reinterpret_cast<const uint4*>(g + h * sd.g_head) : make_uint4(0, 0, 0, 0);
+          const int h = in.h0 + r * S;
+          const bool have = active && h < in.hend;
+          uint4* dst = ring + (slot_in * R + r) * 2 * kQkThreads;
+          qk_copy_async(dst, have ? x + h * sd.x_head : sd.x, have);
+          qk_copy_async(dst + kQkThreads, have ? g + h * sd.g_head : sd.g, have);
         }
+        slot_in = slot_in + 1 == kQkRing ? 0 : slot_in + 1;
+        in.h0 += S * R;
+        if (in.h0 - sub >= in.hend) {
+          in.u += stride;
+          if (in.u < units) in.enter(in.u, chunks, hpu, sd.heads, sub);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int s = 0; s < kQkRing - 1; ++s) copy();
+    long long next = at.u < units ? qk_position(args, at.u / chunks) : 0;
+#pragma unroll 1
+    for (; at.u < units; at.u += stride) {
+      at.enter(at.u, chunks, hpu, sd.heads, sub);
+      const long long pos = next;
+      if (at.u + stride < units) next = qk_position(args, (at.u + stride) / chunks);
+      const bool known = pos >= 0 && pos < args.table_rows;
+      if (!known && lane == 0) report_status(kStatusBadPosition, at.t);
+      QkAngles ang;
+      if (turns && known) qk_load_angles<PAIRS>(args.cos_sin + pos * args.rot, args.rot, i, ang);
+      T* out = static_cast<T*>(sd.out) + at.t * sd.out_row + i;
+#pragma unroll 1
+      for (; at.h0 - sub < at.hend; at.h0 += S * R) {
+        copy();
+        asm volatile("cp.async.wait_group %0;" ::"n"(kQkRing - 1) : "memory");
+        const uint4* row = ring + slot * R * 2 * kQkThreads;
+        slot = slot + 1 == kQkRing ? 0 : slot + 1;
+        if (!known) continue;  // its rows stay unwritten and add nothing
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const int h = h0 + r * S;
+          const int h = at.h0 + r * S;
+          const uint4 xr = row[r * 2 * kQkThreads], gr = row[(r * 2 + 1) * kQkThreads];
           float v[8], gv[8], o[8], ss = 0.f, dot = 0.f;
-          qk_unpack<T>(xr[r], v);
-          qk_unpack<T>(gr[r], gv);
-          qk_partner<T, PAIRS>(gr[r], gv, partner, o);
+          qk_unpack<T>(xr, v);
+          qk_unpack<T>(gr, gv);
+          qk_partner<T, PAIRS>(gr, gv, partner, o);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             gv[j] = fmaf(gv[j], ang.c[j], -(o[j] * ang.s[j]));  // turned back
+            o[j] = gv[j] * v[j];
             ss = fmaf(v[j], v[j], ss);
+            dot = fmaf(o[j], w[j], dot);
           }
+          // Both sums at once; with n = x r: mean(g w n) = r dot / D.
           const float rs = rsqrtf(fmaf(qk_row_sum<L>(ss), inv_dim, args.eps));
+          const float mean = qk_row_sum<L>(dot) * inv_dim * rs;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            v[j] *= rs;  // n
-            dw[j] = fmaf(gv[j], v[j], dw[j]);
-            gv[j] *= w[j];
-            dot = fmaf(gv[j], v[j], dot);
+            dw[j] = fmaf(o[j], rs, dw[j]);
+            gv[j] = rs * (gv[j] * w[j] - v[j] * rs * mean);
           }
-          const float mean = qk_row_sum<L>(dot) * inv_dim;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) gv[j] = rs * (gv[j] - v[j] * mean);
-          if (active && h < hend) *reinterpret_cast<uint4*>(out + h * sd.out_head) = qk_pack<T>(gv);
+          if (active && h < at.hend) *reinterpret_cast<uint4*>(out + h * sd.out_head) = qk_pack<T>(gv);
         }
       }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the ring turns into the sums
+    float* sums = reinterpret_cast<float*>(qk_ring);
+    constexpr int kRow = L * 8 + 1;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sums[warp * S + sub][i + j] = dw[j];
+    for (int j = 0; j < 8; ++j) sums[(warp * S + sub) * kRow + i + j] = dw[j];
     __syncthreads();
     for (int d = threadIdx.x; d < args.dim; d += kQkThreads) {
       float total = 0.f;
 #pragma unroll
-      for (int r = 0; r < kQkWarps * S; ++r) total += sums[r][d];
+      for (int r = 0; r < kQkWarps * S; ++r) total += sums[r * kRow + d];
       args.partials[(static_cast<size_t>(blockIdx.x) * 2 + side) * args.dim + d] = total;
     }
     __syncthreads();

@@ -63,15 +63,20 @@ class AdapterBank:
         if a.dtype != self.dtype or b.dtype != self.dtype:
             raise ValueError(f"the adapter must have the bank's dtype {self.dtype}")
         scale = float(scale)
-        if not math.isfinite(scale) or not math.isfinite(torch.tensor(scale, dtype=torch.float32).item()):
+        if not abs(scale) <= 3.4028234663852886e38:
             raise ValueError("scale must be a finite fp32 value")
-        if not (torch.isfinite(a).all() and torch.isfinite(b).all()):
+        # The largest magnitudes: NaN and infinity stay what they are in a maximum.
+        largest = torch.linalg.vector_norm(a, float("inf")) + torch.linalg.vector_norm(b, float("inf")) * 0
+        if not math.isfinite(largest.item()):
             raise ValueError("the adapter holds values that are not finite")
-        self.unload(slot)
-        self.a[slot, :r].copy_(a)
-        self.b[slot, :r].copy_(b)
-        self.scales[slot] = scale
-        self.ranks[slot] = r
+        into_a, into_b = self.a[slot], self.b[slot]
+        into_a[:r].copy_(a)
+        into_b[:r].copy_(b)
+        if r < self.rank:
+            into_a[r:].zero_()
+            into_b[r:].zero_()
+        self.scales[slot].fill_(scale)
+        self.ranks[slot].fill_(r)
 
     def unload(self, slot):
         slot = self._slot(slot)
