@@ -18,10 +18,10 @@
 // shuffles, and a rotation partner is another lane's register.  A warp takes
 // 32 / L x R x loops heads of one token: the token's angles are loaded once
 // into 16 registers and serve all of them, and R row loads are in flight per
-// lane.  Measured at (32 + 8) heads x 128 bf16 (without overlap of launches):
-// forward of 16384 tokens 77 us with one loop of R = 4, 68 with two, 64 with
-// four (5.4 TB/s with the table; R = 2 70-82); backward of 8192 tokens 70 us
-// with one, 63.5 with two, 65.6 with four (R = 2 68-90).
+// lane.  Measured at (32 + 8) heads x 128 bf16: forward of 16384 tokens 62-63 us,
+// 5.4 TB/s with the table (without overlap of launches: one loop of R = 4 77 us,
+// two 68, four 64; R = 2 70-82); backward of 8192 tokens 57 us, 4.5 TB/s (one
+// loop 64, two 57, four 58; R = 2 58-83; 24 warps an SM instead of 16: 62).
 #pragma once
 
 #include "bokt_device.cuh"
@@ -61,22 +61,43 @@ __device__ __forceinline__ long long qk_position(const QkArgs& a, int t) {
                          : static_cast<long long>(reinterpret_cast<const int32_t*>(a.positions)[t]);
 }
 
+// Two fp32 operations per instruction (sm_100's packed f32x2 arithmetic, each
+// half rounded like the scalar form): both kernels issue more arithmetic per
+// byte than a copy, so this is what keeps them near the memory rate.
+__device__ __forceinline__ unsigned long long qk_bits(float2 a) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ float2 qk_pair(unsigned long long r) {
+  float2 a;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+  return a;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(qk_bits(a)), "l"(qk_bits(b)), "l"(qk_bits(c)));
+  return qk_pair(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(qk_bits(a)), "l"(qk_bits(b)));
+  return qk_pair(r);
+}
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+
 template <typename T>
-__device__ __forceinline__ void qk_unpack(const uint4& v, float (&f)[8]) {
-  float2 p = Pack2<T>::unpack(v.x);
-  f[0] = p.x, f[1] = p.y;
-  p = Pack2<T>::unpack(v.y);
-  f[2] = p.x, f[3] = p.y;
-  p = Pack2<T>::unpack(v.z);
-  f[4] = p.x, f[5] = p.y;
-  p = Pack2<T>::unpack(v.w);
-  f[6] = p.x, f[7] = p.y;
+__device__ __forceinline__ void qk_unpack(const uint4& v, float2 (&f)[4]) {
+  f[0] = Pack2<T>::unpack(v.x);
+  f[1] = Pack2<T>::unpack(v.y);
+  f[2] = Pack2<T>::unpack(v.z);
+  f[3] = Pack2<T>::unpack(v.w);
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 qk_pack(const float (&f)[8]) {
-  return make_uint4(Pack2<T>::pack(f[0], f[1]), Pack2<T>::pack(f[2], f[3]),
-                    Pack2<T>::pack(f[4], f[5]), Pack2<T>::pack(f[6], f[7]));
+__device__ __forceinline__ uint4 qk_pack(const float2 (&f)[4]) {
+  return make_uint4(Pack2<T>::pack(f[0].x, f[0].y), Pack2<T>::pack(f[1].x, f[1].y),
+                    Pack2<T>::pack(f[2].x, f[2].y), Pack2<T>::pack(f[3].x, f[3].y));
 }
 
 template <int L>
@@ -90,10 +111,10 @@ __device__ __forceinline__ float qk_row_sum(float v) {
 // with c[j] and its partner enters with s[j] (the sign of the forward rotation
 // is in s).
 struct QkAngles {
-  float c[8], s[8];
+  float2 c[4], s[4];
   __device__ __forceinline__ QkAngles() {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) c[j] = 1.f, s[j] = 0.f;
+    for (int j = 0; j < 4; ++j) c[j] = both(1.f), s[j] = both(0.f);
   }
 };
 
@@ -105,22 +126,20 @@ __device__ __forceinline__ void qk_load_angles(const float* row, int rot, int i,
     const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      a.c[2 * j] = a.c[2 * j + 1] = cc[j];
-      a.s[2 * j] = -ss[j];
-      a.s[2 * j + 1] = ss[j];
+      a.c[j] = both(cc[j]);
+      a.s[j] = make_float2(-ss[j], ss[j]);
     }
   } else {
     const bool low = i < rot / 2;
     const int f = low ? i : i - rot / 2;
+    const float2 sign = both(low ? -1.f : 1.f);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float4 c = *reinterpret_cast<const float4*>(row + f + 4 * h);
       const float4 s = *reinterpret_cast<const float4*>(row + rot / 2 + f + 4 * h);
-      a.c[4 * h] = c.x, a.c[4 * h + 1] = c.y, a.c[4 * h + 2] = c.z, a.c[4 * h + 3] = c.w;
-      a.s[4 * h] = low ? -s.x : s.x;
-      a.s[4 * h + 1] = low ? -s.y : s.y;
-      a.s[4 * h + 2] = low ? -s.z : s.z;
-      a.s[4 * h + 3] = low ? -s.w : s.w;
+      a.c[2 * h] = make_float2(c.x, c.y), a.c[2 * h + 1] = make_float2(c.z, c.w);
+      a.s[2 * h] = mul2(make_float2(s.x, s.y), sign);
+      a.s[2 * h + 1] = mul2(make_float2(s.z, s.w), sign);
     }
   }
 }
@@ -129,11 +148,11 @@ __device__ __forceinline__ void qk_load_angles(const float* row, int rot, int i,
 // shuffles of packed pairs), or the neighbours of the lane's own pairs.  Lanes
 // past rot are their own partner, with c = 1 and s = 0.
 template <typename T, bool PAIRS>
-__device__ __forceinline__ void qk_partner(const uint4& raw, const float (&v)[8], int partner,
-                                           float (&o)[8]) {
+__device__ __forceinline__ void qk_partner(const uint4& raw, const float2 (&v)[4], int partner,
+                                           float2 (&o)[4]) {
   if constexpr (PAIRS) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = v[j ^ 1];
+    for (int j = 0; j < 4; ++j) o[j] = make_float2(v[j].y, v[j].x);
   } else {
     uint4 p;
     p.x = __shfl_sync(0xffffffffu, raw.x, partner);
@@ -189,25 +208,25 @@ __global__ void __launch_bounds__(kQkThreads, 4) qk_norm_rope_kernel(const QkArg
   QkAngles ang;
   if (turns) qk_load_angles<PAIRS>(args.cos_sin + pos * args.rot, args.rot, i, ang);
   {
-    float w[8], pw[8];
+    float2 w[4], pw[4];
     qk_unpack<T>(wraw, w);
     qk_partner<T, PAIRS>(wraw, w, partner, pw);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ang.c[j] *= w[j], ang.s[j] *= pw[j];
+    for (int j = 0; j < 4; ++j) ang.c[j] = mul2(ang.c[j], w[j]), ang.s[j] = mul2(ang.s[j], pw[j]);
   }
   T* out = static_cast<T*>(sd.out) + t * sd.out_row + i;
   for (;;) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int h = h0 + r * S;
-      float v[8], o[8], ss = 0.f;
+      float2 v[4], o[4], ss = both(0.f);
       qk_unpack<T>(raw[r], v);
       qk_partner<T, PAIRS>(raw[r], v, partner, o);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
-      const float rs = rsqrtf(fmaf(qk_row_sum<L>(ss), inv_dim, args.eps));
+      for (int j = 0; j < 4; ++j) ss = fma2(v[j], v[j], ss);
+      const float2 rs = both(rsqrtf(fmaf(qk_row_sum<L>(ss.x + ss.y), inv_dim, args.eps)));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = fmaf(v[j], ang.c[j], o[j] * ang.s[j]) * rs;
+      for (int j = 0; j < 4; ++j) v[j] = mul2(fma2(v[j], ang.c[j], mul2(o[j], ang.s[j])), rs);
       if (active && h < hend) *reinterpret_cast<uint4*>(out + h * sd.out_head) = qk_pack<T>(v);
     }
     h0 += R * S;
@@ -241,7 +260,7 @@ struct QkWalk {
   }
 };
 
-constexpr int kQkRing = 3;  // batches in flight or in use per warp
+constexpr int kQkRing = 2;  // batches in flight or in use per warp (3 or 4 measured no faster)
 
 // Shared memory of the backward kernel: a ring of R rows of x and of the
 // gradient per lane, and the block's sums.
@@ -279,7 +298,7 @@ __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const 
     const int hpu = S * R * args.loops;
     const int chunks = (sd.heads + hpu - 1) / hpu;
     const int units = args.tokens * chunks;
-    float w[8], dw[8] = {};
+    float2 w[4], dw[4] = {};
     qk_unpack<T>(active && units > 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(sd.w) + i)
                                      : make_uint4(0, 0, 0, 0), w);
     QkWalk in = {}, at = {};  // the batch to copy next, the batch to compute
@@ -317,7 +336,11 @@ __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const 
       const bool known = pos >= 0 && pos < args.table_rows;
       if (!known && lane == 0) report_status(kStatusBadPosition, at.t);
       QkAngles ang;
-      if (turns && known) qk_load_angles<PAIRS>(args.cos_sin + pos * args.rot, args.rot, i, ang);
+      if (turns && known) {
+        qk_load_angles<PAIRS>(args.cos_sin + pos * args.rot, args.rot, i, ang);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ang.s[j] = make_float2(-ang.s[j].x, -ang.s[j].y);  // backwards
+      }
       T* out = static_cast<T*>(sd.out) + at.t * sd.out_row + i;
 #pragma unroll 1
       for (; at.h0 - sub < at.hend; at.h0 += S * R) {
@@ -330,24 +353,25 @@ __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const 
         for (int r = 0; r < R; ++r) {
           const int h = at.h0 + r * S;
           const uint4 xr = row[r * 2 * kQkThreads], gr = row[(r * 2 + 1) * kQkThreads];
-          float v[8], gv[8], o[8], ss = 0.f, dot = 0.f;
+          float2 v[4], gv[4], o[4], ss = both(0.f), dot = both(0.f);
           qk_unpack<T>(xr, v);
           qk_unpack<T>(gr, gv);
           qk_partner<T, PAIRS>(gr, gv, partner, o);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            gv[j] = fmaf(gv[j], ang.c[j], -(o[j] * ang.s[j]));  // turned back
-            o[j] = gv[j] * v[j];
-            ss = fmaf(v[j], v[j], ss);
-            dot = fmaf(o[j], w[j], dot);
+          for (int j = 0; j < 4; ++j) {
+            gv[j] = fma2(gv[j], ang.c[j], mul2(o[j], ang.s[j]));  // turned back
+            o[j] = mul2(gv[j], v[j]);
+            gv[j] = mul2(gv[j], w[j]);
+            ss = fma2(v[j], v[j], ss);
+            dot = fma2(gv[j], v[j], dot);
           }
           // Both sums at once; with n = x r: mean(g w n) = r dot / D.
-          const float rs = rsqrtf(fmaf(qk_row_sum<L>(ss), inv_dim, args.eps));
-          const float mean = qk_row_sum<L>(dot) * inv_dim * rs;
+          const float r1 = rsqrtf(fmaf(qk_row_sum<L>(ss.x + ss.y), inv_dim, args.eps));
+          const float2 rs = both(r1), mean = both(-r1 * inv_dim * qk_row_sum<L>(dot.x + dot.y));
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            dw[j] = fmaf(o[j], rs, dw[j]);
-            gv[j] = rs * (gv[j] * w[j] - v[j] * rs * mean);
+          for (int j = 0; j < 4; ++j) {
+            dw[j] = fma2(o[j], rs, dw[j]);
+            gv[j] = mul2(fma2(mul2(v[j], rs), mean, gv[j]), rs);
           }
           if (active && h < at.hend) *reinterpret_cast<uint4*>(out + h * sd.out_head) = qk_pack<T>(gv);
         }
@@ -358,7 +382,8 @@ __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const 
     float* sums = reinterpret_cast<float*>(qk_ring);
     constexpr int kRow = L * 8 + 1;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sums[(warp * S + sub) * kRow + i + j] = dw[j];
+    for (int j = 0; j < 8; ++j)
+      sums[(warp * S + sub) * kRow + i + j] = j & 1 ? dw[j / 2].y : dw[j / 2].x;
     __syncthreads();
     for (int d = threadIdx.x; d < args.dim; d += kQkThreads) {
       float total = 0.f;
