@@ -152,6 +152,8 @@ _lib = None
 def load():
     """Load (once) and return the ctypes library; raise RuntimeError if absent."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

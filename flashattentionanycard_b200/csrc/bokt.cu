@@ -1835,9 +1835,10 @@ int bokt_moe_decode(const void* x, const void* logits, int logits_dtype, const v
     const void* fn = logits_dtype == BOKT_FP32 ? moe_decode_gate_ptr<float>(E)
                      : logits_dtype == BOKT_BF16 ? moe_decode_gate_ptr<__nv_bfloat16>(E)
                                                  : moe_decode_gate_ptr<__half>(E);
-    const unsigned ctas = unsigned((tokens + 31) / 32);
+    // At least eight tokens to a CTA, at most its sixteen warps.
+    const unsigned ctas = unsigned(tokens >= 8 * bokt::kMdGateCtas ? bokt::kMdGateCtas : (tokens + 7) / 8);
     cudaLaunchAttribute attr[2];
-    cudaLaunchConfig_t lc = launch_config(dim3(ctas), dim3(1024), 0, s, attr);
+    cudaLaunchConfig_t lc = launch_config(dim3(ctas), dim3(bokt::kMdGateThreads), 0, s, attr);
     attr[lc.numAttrs].id = cudaLaunchAttributeClusterDimension;
     attr[lc.numAttrs].val.clusterDim.x = ctas;
     attr[lc.numAttrs].val.clusterDim.y = 1;

@@ -91,29 +91,33 @@ __device__ __forceinline__ float md_value(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
-// One cluster of ceil(T / 32) CTAs, a warp per token, V logits per lane.  Rank
-// 0 gathers the picked ids through distributed shared memory and sorts the
+constexpr int kMdGateThreads = 512;
+constexpr int kMdGateCtas = 8;
+
+// One cluster of up to eight CTAs, a warp per token, V logits per lane.  Rank 0
+// gathers the picked ids through distributed shared memory and sorts the
 // assignments by expert.  The order of one expert's rows follows the atomics
 // and decides nothing: a row's arithmetic does not depend on its place.
+// Latency bound; few warps per SM pick faster than many (64 tokens of 128
+// experts, top 8, on two CTAs of 32 warps: 4.3 us).
 template <typename LT, int V>
-__global__ void __launch_bounds__(1024) moe_decode_gate_kernel(const LT* __restrict__ logits,
-                                                               int renormalize,
-                                                               const MoeDecodeArgs args) {
+__global__ void __launch_bounds__(kMdGateThreads)
+    moe_decode_gate_kernel(const LT* __restrict__ logits, int renormalize, const MoeDecodeArgs args) {
   __shared__ int s_id[kMdMaxTokens * kMdMaxTopk];
+  __shared__ int s_pos[kMdMaxTokens * kMdMaxTopk];
   __shared__ int s_cnt[kMdMaxExperts];
-  __shared__ int s_off[kMdMaxExperts];
-  __shared__ int s_idx[kMdMaxExperts];
-  __shared__ int s_warp[32];
+  __shared__ int s_scan[kMdMaxExperts];  // first row | place among the experts in use << 16
+  __shared__ int s_warp[kMdGateThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int E = args.experts, k = args.topk, T = args.tokens, A = T * k;
-  const uint32_t rank = cluster_ctarank();
-  s_cnt[tid] = 0;
+  const int rank = static_cast<int>(cluster_ctarank());
+  for (int e = tid; e < E; e += kMdGateThreads) s_cnt[e] = 0;
   cluster_sync();  // every CTA runs before another writes its shared memory
   pdl_allow_next();
   pdl_wait();
-  const int t = static_cast<int>(rank) * 32 + warp;
-  int mine = 0;  // lane j: the j-th expert of the token
-  if (t < T) {
+  const int per = (T + gridDim.x - 1) / gridDim.x;  // tokens per CTA, at most 16
+  const int t = rank * per + warp;
+  if (warp < per && t < T) {
     uint32_t key[V], best = 0;
     float sum = 0.f;
 #pragma unroll
@@ -128,7 +132,8 @@ __global__ void __launch_bounds__(1024) moe_decode_gate_kernel(const LT* __restr
       if (i * 32 + lane < E) sum += expf(md_value(key[i]) - mx);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    float gate = 0.f, picked = 0.f;
+    int mine = 0;         // lane j: the j-th expert of the token
+    uint32_t mine_key = 0;
     for (int j = 0; j < k; ++j) {
       best = 0;
 #pragma unroll
@@ -142,13 +147,15 @@ __global__ void __launch_bounds__(1024) moe_decode_gate_kernel(const LT* __restr
 #pragma unroll
       for (int i = 0; i < V; ++i)
         if (i * 32 + lane == at) key[i] = 0u;
-      const float p = expf(md_value(top) - mx) / sum;
-      picked += p;
       if (lane == j) {
         mine = at;
-        gate = p;
+        mine_key = top;
       }
     }
+    const float gate = lane < k ? expf(md_value(mine_key) - mx) / sum : 0.f;
+    float picked = gate;
+#pragma unroll
+    for (int o = kMdMaxTopk / 2; o > 0; o >>= 1) picked += __shfl_xor_sync(0xffffffffu, picked, o);
     if (lane < k) {
       args.gates[t * k + lane] = renormalize ? gate / picked : gate;
       const uint32_t dst = map_shared(smem_addr(&s_id[t * k + lane]), 0);
@@ -156,20 +163,22 @@ __global__ void __launch_bounds__(1024) moe_decode_gate_kernel(const LT* __restr
     }
   }
   if (rank == 0) {
-    for (int i = tid; i < kMdCount1 + args.shares * 4; i += 1024) args.header[i] = 0u;
+    for (int i = tid; i < kMdCount1 + args.shares * 4; i += kMdGateThreads) args.header[i] = 0u;
   }
   cluster_sync();
   if (rank != 0) return;
-  int pos = 0, e = 0;
-  if (tid < A) {
-    e = s_id[tid];
-    pos = atomicAdd(&s_cnt[e], 1);
-  }
+  for (int i = tid; i < A; i += kMdGateThreads) s_pos[i] = atomicAdd(&s_cnt[s_id[i]], 1);
   __syncthreads();
-  // Exclusive scan over experts of (rows, in use), packed 16 + 16 bits.
-  const int c = tid < E ? s_cnt[tid] : 0;
-  const int v = c | (c > 0 ? 1 << 16 : 0);
-  int incl = v;
+  // Exclusive scan over experts of (rows, in use), packed 16 + 16 bits; two
+  // neighbouring experts per thread.
+  static_assert(kMdMaxExperts == 2 * kMdGateThreads, "two experts per thread");
+  int c[2], v[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    c[i] = 2 * tid + i < E ? s_cnt[2 * tid + i] : 0;
+    v[i] = c[i] | (c[i] > 0 ? 1 << 16 : 0);
+  }
+  int incl = v[0] + v[1];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int n = __shfl_up_sync(0xffffffffu, incl, o);
@@ -177,36 +186,32 @@ __global__ void __launch_bounds__(1024) moe_decode_gate_kernel(const LT* __restr
   }
   if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
-  if (warp == 0) {
-    int w = s_warp[lane];
+  int excl = incl - v[0] - v[1], total = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int n = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += n;
-    }
-    s_warp[lane] = w;
+  for (int w = 0; w < kMdGateThreads / 32; ++w) {
+    if (w < warp) excl += s_warp[w];
+    total += s_warp[w];
   }
-  __syncthreads();
-  const int excl = incl - v + (warp > 0 ? s_warp[warp - 1] : 0);
-  if (tid < E) {
-    s_off[tid] = excl & 0xffff;
-    s_idx[tid] = excl >> 16;
-    if (c > 0) {
-      args.act_e[excl >> 16] = tid;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (2 * tid + i < E) s_scan[2 * tid + i] = excl;
+    if (c[i] > 0) {
+      args.act_e[excl >> 16] = 2 * tid + i;
       args.act_off[excl >> 16] = excl & 0xffff;
     }
+    excl += v[i];
   }
   if (tid == 0) {
-    const int active = s_warp[31] >> 16;
+    const int active = total >> 16;
     args.header[kMdActive] = static_cast<uint32_t>(active);
     args.act_off[active] = A;
   }
   __syncthreads();
-  if (tid < A) {
-    const int row = s_off[e] + pos;
-    args.row_token[row] = tid / k;
-    args.row_of[tid] = row;
-    args.act_of[tid] = s_idx[e];
+  for (int i = tid; i < A; i += kMdGateThreads) {
+    const int at = s_scan[s_id[i]], row = (at & 0xffff) + s_pos[i];
+    args.row_token[row] = i / k;
+    args.row_of[i] = row;
+    args.act_of[i] = at >> 16;
   }
 }
 
@@ -389,19 +394,23 @@ __device__ __forceinline__ bool md_combine(const MoeDecodeArgs& args, const MdPl
     }
     const bool in = col < K;
     const int c = col & 255;
-    Vec v[kMdMaxTopk];
+    Vec v[kMdMaxTopk], first_part[kMdMaxTopk];
 #pragma unroll
     for (int j = 0; j < kMdMaxTopk; ++j) {
-      const int r = __shfl_sync(0xffffffffu, slot.row, j);
+      const int r = __shfl_sync(0xffffffffu, slot.row, j), b = __shfl_sync(0xffffffffu, slot.base, j);
+      const int s0 = __shfl_sync(0xffffffffu, slot.g0, j), s1 = __shfl_sync(0xffffffffu, slot.g1, j);
       v[j].zero();
+      first_part[j].zero();
       if (j < topk && in) v[j].load(args.y + static_cast<size_t>(r) * K + col);
+      if (j < topk && s0 <= s1) first_part[j].load(args.part + 2 * s0 * slot_floats + b * 256 + c);
     }
 #pragma unroll
     for (int j = 0; j < kMdMaxTopk; ++j) {
       if (j >= topk) break;
       const int b = __shfl_sync(0xffffffffu, slot.base, j);
       const int s0 = __shfl_sync(0xffffffffu, slot.g0, j), s1 = __shfl_sync(0xffffffffu, slot.g1, j);
-      for (int s = s0; s <= s1; s += 4) {
+      v[j].add(first_part[j]);
+      for (int s = s0 + 1; s <= s1; s += 4) {
         Vec w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -754,36 +763,63 @@ __global__ void __launch_bounds__(kMdThreads, 1)
               done = true;
               __threadfence();
               // Share s0 starts at or before the tile: slot 2 s0 + 1; the others
-              // 2 s.  Eight rows of two shares in flight at a time.
-              for (int r0 = 0; r0 < m; r0 += 8) {
-                float g[8] = {}, uu[8] = {};
-                for (int s = s0; s <= s1; s += 2) {
-                  const float* p0 = args.part + (2 * s + (s == s0)) * slot_floats + lcol;
-                  const float* p1 = args.part + 2 * min(s + 1, s1) * slot_floats + lcol;
-                  float v[8][4];
+              // 2 s.  32 loads in flight: one row of sixteen shares, or eight
+              // rows of two.
+              const float* from = args.part + lcol;
+              auto slot_of = [&](int s) { return from + (2 * s + (s == s0)) * slot_floats; };
+              auto finish = [&](int r, float g, float u) {
+                if (col < I)
+                  h[static_cast<size_t>(row0 + r) * I + col] =
+                      Pack2<T>::from_float(g / (1.f + expf(-g)) * u);
+              };
+              if (m <= 2) {
+                for (int r = 0; r < m; ++r) {
+                  float g = 0.f, uu = 0.f;
+                  for (int s = s0; s <= s1; s += 16) {
+                    float v[16][2];
 #pragma unroll
-                  for (int r = 0; r < 8; ++r) {
-                    const int at = min(r0 + r, m - 1) * 256;
-                    v[r][0] = __ldcg(p0 + at);
-                    v[r][1] = __ldcg(p0 + at + 128);
-                    v[r][2] = __ldcg(p1 + at);
-                    v[r][3] = __ldcg(p1 + at + 128);
+                    for (int i = 0; i < 16; ++i) {
+                      v[i][0] = s + i <= s1 ? __ldcg(slot_of(s + i) + r * 256) : 0.f;
+                      v[i][1] = s + i <= s1 ? __ldcg(slot_of(s + i) + r * 256 + 128) : 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                      if (s + i <= s1) {
+                        g += v[i][0];
+                        uu += v[i][1];
+                      }
                   }
+                  finish(r, g, uu);
+                }
+              } else {
+                for (int r0 = 0; r0 < m; r0 += 8) {
+                  float g[8] = {}, uu[8] = {};
+                  for (int s = s0; s <= s1; s += 2) {
+                    const float* p0 = slot_of(s);
+                    const float* p1 = slot_of(min(s + 1, s1));
+                    float v[8][4];
 #pragma unroll
-                  for (int r = 0; r < 8; ++r) {
-                    g[r] += v[r][0];
-                    uu[r] += v[r][1];
-                    if (s < s1) {
-                      g[r] += v[r][2];
-                      uu[r] += v[r][3];
+                    for (int r = 0; r < 8; ++r) {
+                      const int at = min(r0 + r, m - 1) * 256;
+                      v[r][0] = __ldcg(p0 + at);
+                      v[r][1] = __ldcg(p0 + at + 128);
+                      v[r][2] = __ldcg(p1 + at);
+                      v[r][3] = __ldcg(p1 + at + 128);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                      g[r] += v[r][0];
+                      uu[r] += v[r][1];
+                      if (s < s1) {
+                        g[r] += v[r][2];
+                        uu[r] += v[r][3];
+                      }
                     }
                   }
-                }
 #pragma unroll
-                for (int r = 0; r < 8; ++r)
-                  if (r0 + r < m && col < I)
-                    h[static_cast<size_t>(row0 + r0 + r) * I + col] =
-                        Pack2<T>::from_float(g[r] / (1.f + expf(-g[r])) * uu[r]);
+                  for (int r = 0; r < 8; ++r)
+                    if (r0 + r < m) finish(r0 + r, g[r], uu[r]);
+                }
               }
             }
           }

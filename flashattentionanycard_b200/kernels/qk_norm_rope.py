@@ -48,23 +48,28 @@ def rope_table(rows, rot, base=10000.0, device="cuda"):
 _Strides = ctypes.c_int64 * 12
 
 
-def _view(name, x, shape, dtype, index, writes):
-    """Checks one [T, heads, D] view; returns its row and head strides."""
-    if x.shape != shape:
-        raise ValueError(f"shape mismatch: {name} {tuple(x.shape)}, expected {tuple(shape)}")
-    if x.dtype != dtype:
-        raise ValueError(f"{name} must share q's dtype")
-    row, head, last = x.stride()
+def _views(named, shape, dtype, index):
+    """Checks views of one shape, (name, view, written) each; returns their row
+    and head strides in order."""
     n, h, d = shape
-    if last != 1 and d > 1:
-        raise ValueError(f"{name} must be contiguous in its last dimension")
-    # Distinct elements of an output must be distinct memory.
-    if writes and not ((head >= d and row >= head * (h - 1) + d) or (row >= d and head >= row * (n - 1) + d)
-                       or n * h <= 1 or (n == 1 and head >= d) or (h == 1 and row >= d)):
-        raise ValueError(f"{name} must not overlap itself (strides {x.stride()})")
-    if x.get_device() != index:
-        raise ValueError("all tensors must be on one CUDA device")
-    return row, head
+    out = []
+    for name, x, written in named:
+        if x.shape != shape:
+            raise ValueError(f"shape mismatch: {name} {tuple(x.shape)}, expected {tuple(shape)}")
+        if x.dtype != dtype:
+            raise ValueError(f"{name} must share q's dtype")
+        row, head, last = x.stride()
+        if last != 1 and d > 1:
+            raise ValueError(f"{name} must be contiguous in its last dimension")
+        # Distinct elements of an output must be distinct memory.
+        if written and not (
+                (head >= d and row >= head * (h - 1) + d) or (row >= d and head >= row * (n - 1) + d)
+                or n * h <= 1 or (n == 1 and head >= d) or (h == 1 and row >= d)):
+            raise ValueError(f"{name} must not overlap itself (strides {x.stride()})")
+        if x.get_device() != index:
+            raise ValueError("all tensors must be on one CUDA device")
+        out += (row, head)
+    return out
 
 
 def _weight(name, w, d, dtype, index):
@@ -110,9 +115,8 @@ def launch(q, k, q_weight, k_weight, positions, cos_sin, q_out, k_out, epsilon=1
     """q_out, k_out = rotated norms of q's and k's heads (q_out may be q, k_out may be k)."""
     qs, ks, rot, rows, index, i64 = _check(q, k, q_weight, k_weight, positions, cos_sin, epsilon)
     dtype = q.dtype
-    strides = _Strides(
-        *_view("q", q, qs, dtype, index, False), *_view("q_out", q_out, qs, dtype, index, True),
-        *_view("k", k, ks, dtype, index, False), *_view("k_out", k_out, ks, dtype, index, True))
+    strides = _Strides(*_views((("q", q, False), ("q_out", q_out, True)), qs, dtype, index),
+                       *_views((("k", k, False), ("k_out", k_out, True)), ks, dtype, index))
     if index < 0:
         raise ValueError("q, k and their tensors must be CUDA tensors")
     lib = _native.load()
@@ -135,10 +139,8 @@ def launch_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, cos_sin
     qs, ks, rot, rows, index, i64 = _check(q, k, q_weight, k_weight, positions, cos_sin, epsilon)
     dtype, d = q.dtype, qs[2]
     strides = _Strides(
-        *_view("q", q, qs, dtype, index, False), *_view("dq", dq, qs, dtype, index, True),
-        *_view("dq_out", dq_out, qs, dtype, index, False),
-        *_view("k", k, ks, dtype, index, False), *_view("dk", dk, ks, dtype, index, True),
-        *_view("dk_out", dk_out, ks, dtype, index, False))
+        *_views((("q", q, False), ("dq", dq, True), ("dq_out", dq_out, False)), qs, dtype, index),
+        *_views((("k", k, False), ("dk", dk, True), ("dk_out", dk_out, False)), ks, dtype, index))
     _weight("dq_weight", dq_weight, d, torch.float32, index)
     _weight("dk_weight", dk_weight, d, torch.float32, index)
     if index < 0:
