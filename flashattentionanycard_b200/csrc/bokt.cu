@@ -18,6 +18,7 @@
 #include "gemm_tc2.cuh"
 #include "lora_gemm.cuh"
 #include "moe_decode.cuh"
+#include "moe_few.cuh"
 #include "moe_route.cuh"
 #include "norm_gemm.cuh"
 #include "qk_norm_rope.cuh"
@@ -1690,6 +1691,19 @@ int bokt_rope_table(float* cos_sin, int rows, int rot, double base, void* stream
 // ----------------------------------------------------------------- MoE layer for a few tokens
 namespace {
 
+cudaError_t launch_cluster(const void* fn, int grid, int threads, int smem, int cluster,
+                           cudaStream_t s, void** kargs) {
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t lc = launch_config(dim3(unsigned(grid)), dim3(unsigned(threads)), smem, s, attr);
+  attr[lc.numAttrs].id = cudaLaunchAttributeClusterDimension;
+  attr[lc.numAttrs].val.clusterDim.x = unsigned(cluster);
+  attr[lc.numAttrs].val.clusterDim.y = 1;
+  attr[lc.numAttrs].val.clusterDim.z = 1;
+  lc.numAttrs += 1;
+  return cudaLaunchKernelExC(&lc, fn, kargs);
+}
+
+
 // Byte offsets of the workspace's parts, each 256-byte aligned.
 struct MoeDecodeLayout {
   int shares;
@@ -1731,12 +1745,38 @@ int moe_decode_layout(int tokens, int E, int K, int I, int topk, const DeviceInf
   return BOKT_OK;
 }
 
-template <typename LT>
 const void* moe_decode_gate_ptr(int E) {
-  if (E <= 32) return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<LT, 1>);
-  if (E <= 128) return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<LT, 4>);
-  if (E <= 256) return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<LT, 8>);
-  return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<LT, 32>);
+  if (E <= 32) return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<1>);
+  if (E <= 128) return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<4>);
+  if (E <= 256) return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<8>);
+  return reinterpret_cast<const void*>(&bokt::moe_decode_gate_kernel<32>);
+}
+
+template <typename T>
+const void* moe_few_ptr(bool down, int E) {
+  if (down)
+    return E <= 128 ? reinterpret_cast<const void*>(&bokt::moe_few_down_kernel<T, 4>)
+                    : reinterpret_cast<const void*>(&bokt::moe_few_down_kernel<T, 32>);
+  return E <= 128 ? reinterpret_cast<const void*>(&bokt::moe_few_up_kernel<T, 4>)
+                  : reinterpret_cast<const void*>(&bokt::moe_few_up_kernel<T, 32>);
+}
+
+// Weight bytes (of the experts that may be in use) up to which a handful of
+// tokens takes the two-kernel chain instead of the persistent stream.
+constexpr long long kFewBytes = 1ll << 40;
+
+// Cluster sizes of the two kernels, or false: the persistent kernel's case.
+bool moe_few_plan(int tokens, int E, int K, int I, int topk, const DeviceInfo& dev, int* up, int* down) {
+  if (tokens > bokt::kFewTokens) return false;
+  const long long active = E < tokens * topk ? E : tokens * topk;  // at most
+  if (active * 6 * K * I > kFewBytes) return false;
+  const long long tiles1 = active * ((I + 127) / 128), tiles2 = (K + 127) / 128;
+  const int ksteps = (K + 63) / 64, units = topk * ((I + 127) / 128);  // units: at least
+  *up = *down = 1;
+  while (*up < 8 && tiles1 * *up * 2 <= dev.sm_count && ksteps >= *up * 2) *up *= 2;
+  while (*down < 8 && tiles2 * *down * 2 <= dev.sm_count && units >= *down * 2) *down *= 2;
+  // A CTA of the second kernel keeps an accumulator for every expert of its run.
+  return (active + *down - 1) / *down + 1 <= bokt::kFewExperts;
 }
 
 }  // namespace
@@ -1831,10 +1871,30 @@ int bokt_moe_decode(const void* x, const void* logits, int logits_dtype, const v
     if ((rc = encode_map(&mh, a.h, 2, d, st, b, fp16))) return rc;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int up = 1, down = 1;
+  if (moe_few_plan(tokens, E, K, I, topk, dev, &up, &down)) {
+    bokt::MoeFewArgs f = {};
+    f.logits = logits, f.logits_dtype = logits_dtype, f.renormalize = renormalize ? 1 : 0;
+    f.tokens = tokens, f.experts = E, f.k = K, f.inner = I, f.topk = topk;
+    f.idesc = bokt::make_idesc_f16_swapped(uint32_t(dtype), 16);
+    f.h = a.h, f.out = out;
+    const long long active = E < A ? E : A;
+    for (int i = 0; i < 2; ++i) {
+      const void* fn = fp16 ? moe_few_ptr<__half>(i, E) : moe_few_ptr<__nv_bfloat16>(i, E);
+      const int smem_few = bokt::moe_few_smem_bytes(i ? bokt::kFewDownStage : bokt::kFewUpStage);
+      if ((rc = ensure_smem(fn, smem_few)) || (rc = ensure_carveout(fn))) return rc;
+      f.cluster = i ? down : up;
+      const long long grid = f.cluster * (i ? (K + 127) / 128 : active * ((I + 127) / 128));
+      void* up_args[] = {&mg, &mx, &f};
+      void* down_args[] = {&md, &mh, &f};
+      cudaError_t e = launch_cluster(fn, int(grid), bokt::kFewThreads, smem_few, f.cluster, s,
+                                     i ? down_args : up_args);
+      if (e != cudaSuccess) return cuda_fail(e, "moe_few launch");
+    }
+    return BOKT_OK;
+  }
   {
-    const void* fn = logits_dtype == BOKT_FP32 ? moe_decode_gate_ptr<float>(E)
-                     : logits_dtype == BOKT_BF16 ? moe_decode_gate_ptr<__nv_bfloat16>(E)
-                                                 : moe_decode_gate_ptr<__half>(E);
+    const void* fn = moe_decode_gate_ptr(E);
     // At least eight tokens to a CTA, at most its sixteen warps.
     const unsigned ctas = unsigned(tokens >= 8 * bokt::kMdGateCtas ? bokt::kMdGateCtas : (tokens + 7) / 8);
     cudaLaunchAttribute attr[2];
@@ -1846,7 +1906,7 @@ int bokt_moe_decode(const void* x, const void* logits, int logits_dtype, const v
     lc.numAttrs += 1;
     if ((rc = ensure_carveout(fn))) return rc;
     int renorm = renormalize ? 1 : 0;
-    void* kargs[] = {const_cast<void*>(static_cast<const void*>(&logits)), &renorm, &a};
+    void* kargs[] = {&logits, &logits_dtype, &renorm, &a};
     cudaError_t e = cudaLaunchKernelExC(&lc, fn, kargs);
     if (e != cudaSuccess) return cuda_fail(e, "moe_decode_gate launch");
   }
@@ -1965,18 +2025,6 @@ int lora_plan(int M, int N, int K, int slots, int rank, const DeviceInfo& dev, L
   p->total = p->h + up(groups * p->tile_rows * 64 * 2);
   if (p->total < 256) p->total = 256;
   return BOKT_OK;
-}
-
-cudaError_t launch_cluster(const void* fn, int grid, int threads, int smem, int cluster,
-                           cudaStream_t s, void** kargs) {
-  cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t lc = launch_config(dim3(unsigned(grid)), dim3(unsigned(threads)), smem, s, attr);
-  attr[lc.numAttrs].id = cudaLaunchAttributeClusterDimension;
-  attr[lc.numAttrs].val.clusterDim.x = unsigned(cluster);
-  attr[lc.numAttrs].val.clusterDim.y = 1;
-  attr[lc.numAttrs].val.clusterDim.z = 1;
-  lc.numAttrs += 1;
-  return cudaLaunchKernelExC(&lc, fn, kargs);
 }
 
 template <typename T>

@@ -91,6 +91,59 @@ __device__ __forceinline__ float md_value(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
+__device__ __forceinline__ float md_logit(const void* logits, int dtype, size_t at) {
+  if (dtype == 2) return static_cast<const float*>(logits)[at];
+  if (dtype == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(logits)[at]);
+  return __half2float(static_cast<const __half*>(logits)[at]);
+}
+
+// The top k of one token's softmax, one warp, V logits per lane (V * 32 >= E):
+// lane j < k returns the j-th expert and its gate.  dtype: BOKT_FP16/BF16/FP32.
+template <int V>
+__device__ __forceinline__ int md_pick(const void* logits, int dtype, int t, int E, int k,
+                                       int renormalize, int lane, float* gate_out) {
+  uint32_t key[V], best = 0;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = i * 32 + lane;
+    key[i] = e < E ? md_key(md_logit(logits, dtype, static_cast<size_t>(t) * E + e)) : 0u;
+    best = max(best, key[i]);
+  }
+  const float mx = md_value(__reduce_max_sync(0xffffffffu, best));
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i * 32 + lane < E) sum += expf(md_value(key[i]) - mx);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  int mine = 0;
+  uint32_t mine_key = 0;
+  for (int j = 0; j < k; ++j) {
+    best = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) best = max(best, key[i]);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int i = V - 1; i >= 0; --i)
+      if (key[i] == top) at = i * 32 + lane;
+    at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i * 32 + lane == at) key[i] = 0u;
+    if (lane == j) {
+      mine = at;
+      mine_key = top;
+    }
+  }
+  const float gate = lane < k ? expf(md_value(mine_key) - mx) / sum : 0.f;
+  float picked = gate;
+#pragma unroll
+  for (int o = kMdMaxTopk / 2; o > 0; o >>= 1) picked += __shfl_xor_sync(0xffffffffu, picked, o);
+  *gate_out = renormalize ? gate / picked : gate;
+  return mine;
+}
+
 constexpr int kMdGateThreads = 512;
 constexpr int kMdGateCtas = 8;
 
@@ -100,9 +153,10 @@ constexpr int kMdGateCtas = 8;
 // and decides nothing: a row's arithmetic does not depend on its place.
 // Latency bound; few warps per SM pick faster than many (64 tokens of 128
 // experts, top 8, on two CTAs of 32 warps: 4.3 us).
-template <typename LT, int V>
+template <int V>
 __global__ void __launch_bounds__(kMdGateThreads)
-    moe_decode_gate_kernel(const LT* __restrict__ logits, int renormalize, const MoeDecodeArgs args) {
+    moe_decode_gate_kernel(const void* __restrict__ logits, int logits_dtype, int renormalize,
+                           const MoeDecodeArgs args) {
   __shared__ int s_id[kMdMaxTokens * kMdMaxTopk];
   __shared__ int s_pos[kMdMaxTokens * kMdMaxTopk];
   __shared__ int s_cnt[kMdMaxExperts];
@@ -118,46 +172,10 @@ __global__ void __launch_bounds__(kMdGateThreads)
   const int per = (T + gridDim.x - 1) / gridDim.x;  // tokens per CTA, at most 16
   const int t = rank * per + warp;
   if (warp < per && t < T) {
-    uint32_t key[V], best = 0;
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = i * 32 + lane;
-      key[i] = e < E ? md_key(static_cast<float>(logits[static_cast<size_t>(t) * E + e])) : 0u;
-      best = max(best, key[i]);
-    }
-    const float mx = md_value(__reduce_max_sync(0xffffffffu, best));
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i * 32 + lane < E) sum += expf(md_value(key[i]) - mx);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    int mine = 0;         // lane j: the j-th expert of the token
-    uint32_t mine_key = 0;
-    for (int j = 0; j < k; ++j) {
-      best = 0;
-#pragma unroll
-      for (int i = 0; i < V; ++i) best = max(best, key[i]);
-      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-      int at = 0x7fffffff;
-#pragma unroll
-      for (int i = V - 1; i >= 0; --i)
-        if (key[i] == top) at = i * 32 + lane;
-      at = __reduce_min_sync(0xffffffffu, at);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i * 32 + lane == at) key[i] = 0u;
-      if (lane == j) {
-        mine = at;
-        mine_key = top;
-      }
-    }
-    const float gate = lane < k ? expf(md_value(mine_key) - mx) / sum : 0.f;
-    float picked = gate;
-#pragma unroll
-    for (int o = kMdMaxTopk / 2; o > 0; o >>= 1) picked += __shfl_xor_sync(0xffffffffu, picked, o);
+    float gate;
+    const int mine = md_pick<V>(logits, logits_dtype, t, E, k, renormalize, lane, &gate);
     if (lane < k) {
-      args.gates[t * k + lane] = renormalize ? gate / picked : gate;
+      args.gates[t * k + lane] = gate;
       const uint32_t dst = map_shared(smem_addr(&s_id[t * k + lane]), 0);
       asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(mine) : "memory");
     }
