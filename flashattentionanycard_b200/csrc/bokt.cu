@@ -1761,20 +1761,20 @@ const void* moe_few_ptr(bool down, int E) {
                   : reinterpret_cast<const void*>(&bokt::moe_few_up_kernel<T, 32>);
 }
 
-// Weight bytes (of the experts that may be in use) up to which a handful of
-// tokens takes the two-kernel chain instead of the persistent stream.
-constexpr long long kFewBytes = 1ll << 40;
-
-// Cluster sizes of the two kernels, or false: the persistent kernel's case.
+// Cluster sizes of the two kernels for a handful of tokens, or false: the
+// persistent kernel's case.
 bool moe_few_plan(int tokens, int E, int K, int I, int topk, const DeviceInfo& dev, int* up, int* down) {
-  if (tokens > bokt::kFewTokens) return false;
+  if (tokens > bokt::kFewTokens || tokens * topk > bokt::kFewRows) return false;
   const long long active = E < tokens * topk ? E : tokens * topk;  // at most
-  if (active * 6 * K * I > kFewBytes) return false;
   const long long tiles1 = active * ((I + 127) / 128), tiles2 = (K + 127) / 128;
-  const int ksteps = (K + 63) / 64, units = topk * ((I + 127) / 128);  // units: at least
+  const int ksteps = (K + 63) / 64, steps2 = (I + 127) / 128;
   *up = *down = 1;
   while (*up < 8 && tiles1 * *up * 2 <= dev.sm_count && ksteps >= *up * 2) *up *= 2;
-  while (*down < 8 && tiles2 * *down * 2 <= dev.sm_count && units >= *down * 2) *down *= 2;
+  while (*down < 8 && tiles2 * *down * 2 <= dev.sm_count && topk * steps2 >= *down * 2) *down *= 2;
+  // The second kernel has one cluster per 128 columns of out: with few of them
+  // and long runs the persistent kernel's even shares are faster (16 tokens of
+  // 64 experts x [1024, 2 x 1024], 64 steps a CTA: 58 us, here 74).
+  if (tiles2 * *down * 2 < dev.sm_count && active * steps2 > 32 * *down) return false;
   // A CTA of the second kernel keeps an accumulator for every expert of its run.
   return (active + *down - 1) / *down + 1 <= bokt::kFewExperts;
 }

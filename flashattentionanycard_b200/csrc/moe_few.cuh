@@ -1,5 +1,5 @@
-// The MoE layer of moe_decode.cuh for a handful of tokens (at most 16): two
-// kernels whose boundary takes the place of the persistent kernel's counters.
+// The MoE layer of moe_decode.cuh for a handful of tokens (at most 16, and 64
+// assignments): two kernels whose boundary takes the place of the persistent kernel's counters.
 //
 // With few tokens and small experts the layer is a chain of latencies, not a
 // stream: route, first weights, reduce, hand h over, reduce, combine.  So here
@@ -14,8 +14,12 @@
 // moe_few_down  out: 128 columns a cluster; its k-steps run over the experts in
 //               use, each with 16 accumulator columns of its own; a CTA weighs
 //               its rows by their gates before the cluster's sum.
-// Both sums run in rank order.  One token, 8 experts x [1024, 2 x 2048], top 2:
-// see moe_decode.cuh's 22.7 us.
+// Both sums run in rank order.  Measured against the persistent kernel (us a
+// call): 8 experts x [1024, 2 x 2048], top 2: one token 13.2 and 22.7, four 25
+// and 33, sixteen 33 and 35; 128 x [2048, 2 x 768], top 8: one token 24 and 40,
+// four 58 and 67; 16 x [4096, 2 x 14336], top 2: one token 122 and 123.  Past 16
+// tokens routing in every CTA costs more than it saves (37 tokens of 12 experts:
+// 45 and 35).
 #pragma once
 
 #include "moe_decode.cuh"
@@ -23,7 +27,7 @@
 namespace bokt {
 
 constexpr int kFewTokens = 16;
-constexpr int kFewRows = kFewTokens * kMdMaxTopk;  // assignments
+constexpr int kFewRows = 64;  // assignments
 constexpr int kFewThreads = 256;
 constexpr int kFewStages = 3;
 constexpr int kFewTmemCols = 256;                  // moe_few_down: 16 experts a CTA
@@ -52,7 +56,7 @@ struct FewRoute {
   int place[kFewRows];   // a of an assignment
   int row[kFewRows];     // row of an assignment
   int token[kFewRows];   // token of a row
-  int warp_leads[4];
+  int warp_leads[2];
 };
 
 template <int V>
@@ -88,7 +92,7 @@ __device__ __forceinline__ void few_route(const MoeFewArgs& args, FewRoute& r) {
       r.expert[a] = r.id[tid];
       r.place[tid] = a;
     }
-    if (tid == 0) r.active = r.warp_leads[0] + r.warp_leads[1] + r.warp_leads[2] + r.warp_leads[3];
+    if (tid == 0) r.active = r.warp_leads[0] + r.warp_leads[1];
   }
   __syncthreads();
   if (tid < A && !leads) {
