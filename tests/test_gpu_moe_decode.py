@@ -90,6 +90,9 @@ SHAPES = [
     (31, 33, 520, 264, 5), (33, 12, 1032, 1000, 3), (48, 40, 136, 328, 6), (64, 130, 256, 96, 8),
     (100, 2, 128, 520, 2), (128, 8, 512, 256, 2), (128, 300, 64, 24, 8), (65, 1024, 72, 16, 7),
     (1, 16, 2048, 4096, 8), (5, 4, 4096, 8, 1), (5, 4, 8, 4096, 2),
+    # sixteen tokens and fewer on either kernel: more assignments, long runs, wide outputs
+    (9, 64, 128, 72, 8), (16, 64, 256, 1024, 4), (16, 3, 2056, 136, 2), (8, 40, 4104, 24, 8),
+    (13, 600, 264, 40, 4), (2, 2, 20000, 16, 2),
 ]
 
 
@@ -117,7 +120,7 @@ def test_gate_types_ties_and_renormalisation(logits, renormalize, cuda_device):
     check(a, 4, out, "bf16", renormalize)
 
 
-@pytest.mark.parametrize("t, skew", [(128, 100.0), (37, 3.0)])
+@pytest.mark.parametrize("t, skew", [(128, 100.0), (37, 3.0), (16, 100.0), (5, 3.0)])
 def test_one_hot_expert(t, skew, cuda_device):
     a = make(t, 9, 200, 72, skew=skew)
     check(a, 3, run(a, 3), "bf16")
@@ -130,8 +133,9 @@ def test_fewer_finite_logits_than_picks(cuda_device):
     check(a, 3, run(a, 3), "bf16")
 
 
-def test_rows_without_a_distribution_are_nan_and_alone(cuda_device):
-    a = make(20, 6, 64, 32)
+@pytest.mark.parametrize("t", [20, 14])
+def test_rows_without_a_distribution_are_nan_and_alone(t, cuda_device):
+    a = make(t, 6, 64, 32)
     clean = run(a, 2)
     a["logits"][3] = float("-inf")
     a["logits"][7, 2] = float("nan")
@@ -140,7 +144,7 @@ def test_rows_without_a_distribution_are_nan_and_alone(cuda_device):
     a["x"][12, 5] = float("inf")
     out = run(a, 2)
     bad = [3, 7, 9, 11]
-    good = [i for i in range(20) if i not in bad + [12]]
+    good = [i for i in range(t) if i not in bad + [12]]
     assert torch.isnan(out[bad]).all()
     assert not torch.isfinite(out[12]).any()
     assert torch.equal(out[good], clean[good])
@@ -157,8 +161,9 @@ def test_experts_nobody_picked_are_not_touched(cuda_device):
     assert torch.equal(run(a, 2), clean)
 
 
-def test_weights_that_are_not_finite_reach_their_tokens_only(cuda_device):
-    a = make(30, 4, 64, 136)
+@pytest.mark.parametrize("t", [30, 15])
+def test_weights_that_are_not_finite_reach_their_tokens_only(t, cuda_device):
+    a = make(t, 4, 64, 136)
     clean = run(a, 1)
     a["w_gate_up"][2] = float("nan")
     out = run(a, 1)
@@ -171,16 +176,17 @@ def test_no_tokens(cuda_device):
     assert run(a, 2).shape == (0, 64)
 
 
-def test_dirty_workspace_and_guard_bytes(cuda_device):
-    a = make(23, 10, 264, 136)
+@pytest.mark.parametrize("t", [23, 11])
+def test_dirty_workspace_and_guard_bytes(t, cuda_device):
+    a = make(t, 10, 264, 136)
     want = run(a, 3)
-    need = moe_decode.workspace_bytes(23, 10, 264, 136, 3)
+    need = moe_decode.workspace_bytes(t, 10, 264, 136, 3)
     for fill in (0, 255, 127):
         ws = torch.full((need + 4096,), fill, dtype=torch.uint8, device=cuda_device)
         out = torch.zeros(40, 264, dtype=torch.bfloat16, device=cuda_device)
-        moe_decode.launch(**a, out=out[8:31], topk=3, workspace=ws[:need])
-        assert torch.equal(out[8:31], want)
-        assert not out[:8].any() and not out[31:].any() and (ws[need:] == fill).all()
+        moe_decode.launch(**a, out=out[8:8 + t], topk=3, workspace=ws[:need])
+        assert torch.equal(out[8:8 + t], want)
+        assert not out[:8].any() and not out[8 + t:].any() and (ws[need:] == fill).all()
     with pytest.raises(ValueError, match="workspace"):
         run(a, 3, workspace=ws[:need - 1])
     with pytest.raises(RuntimeError, match="aligned"):
