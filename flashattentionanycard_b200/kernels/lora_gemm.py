@@ -121,13 +121,16 @@ def launch(x, w, bank, ids, out, workspace=None):
     index = x.get_device()
     if index < 0 or not (w.get_device() == out.get_device() == ids.get_device() == bank.a.get_device() == index):
         raise ValueError("all tensors and the bank must be on one CUDA device")
+    xp, outp = x.data_ptr(), out.data_ptr()
+    if xp < outp + 2 * m * n and outp < xp + 2 * m * k:
+        raise ValueError("out must not overlap x: finished columns are written while others still read x")
     lib = _native.load()
     with _native.on_device(index):
         scratch, nbytes = _native.workspace("bokt_lora_gemm_workspace_bytes", (m, n, k, bank.slots, bank.rank),
                                             index, workspace)
         rc = lib.bokt_lora_gemm(
-            x.data_ptr(), w.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
-            bank.ranks.data_ptr(), ids.data_ptr(), out.data_ptr(), m, n, k, bank.slots, bank.rank,
+            xp, w.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
+            bank.ranks.data_ptr(), ids.data_ptr(), outp, m, n, k, bank.slots, bank.rank,
             _native.dtype_code(dtype), scratch.data_ptr(), nbytes, _native.current_stream(index))
     _native.check(rc, "bokt_lora_gemm")
     return out

@@ -31,7 +31,8 @@ def workspace_bytes(tokens, experts, k, inner, topk):
 
 
 def launch(x, logits, w_gate_up, w_down, out, topk, renormalize=True, workspace=None):
-    """out[T, K] = the layer's output for x [T, K] and logits [T, E] (T <= 128).
+    """out[T, K] = the layer's output for x [T, K] and logits [T, E] (T <= 128);
+    out may be x itself.
 
     ``workspace``: a uint8 tensor of ``workspace_bytes`` (calls that may overlap
     on the GPU need one each); by default the call takes a fresh one from

@@ -143,6 +143,8 @@ def launch_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, cos_sin
         *_views((("k", k, False), ("dk", dk, True), ("dk_out", dk_out, False)), ks, dtype, index))
     _weight("dq_weight", dq_weight, d, torch.float32, index)
     _weight("dk_weight", dk_weight, d, torch.float32, index)
+    if abs(dq_weight.data_ptr() - dk_weight.data_ptr()) < 4 * d:
+        raise ValueError("dq_weight and dk_weight must be separate buffers (add them where q and k share a weight)")
     if index < 0:
         raise ValueError("q, k and their tensors must be CUDA tensors")
     lib = _native.load()

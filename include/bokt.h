@@ -215,8 +215,8 @@ int bokt_rmsnorm_gemm(const void* X, const void* B_folded, void* C, float* row_s
  * own rank (rows past it are zero), 0 for an empty slot; ids int32 [M].  The
  * adapters in use are read once per row tile and join the projection's fp32
  * accumulator; scales[a] (x A_a^T) is rounded to the type (it is a tensor-core
- * operand), the sum once.  lora_b must be finite: rows of other adapters
- * multiply it by zero.  An id outside [-1, slots) or of an empty slot sets the
+ * operand), the sum once.  out must not overlap x.  lora_b must be finite:
+ * rows of other adapters multiply it by zero.  An id outside [-1, slots) or of an empty slot sets the
  * device status word (code 6) and its row gets x W alone.  rank: 16, 32, 64 or
  * 128; slots <= 1024; K and N multiples of 8; 16-byte aligned pointers.
  * workspace: bokt_lora_gemm_workspace_bytes(...) bytes of device scratch,
@@ -256,7 +256,7 @@ int bokt_qk_norm_rope(const void* q, const void* k, const void* q_weight, const 
 
 /*
  * Gradients of bokt_qk_norm_rope: dq, dk (may be dq_out / dk_out themselves)
- * and the weights' gradients dq_weight, dk_weight (fp32 [dim], overwritten;
+ * and the weights' gradients dq_weight, dk_weight (fp32 [dim], apart, overwritten;
  * summed in a fixed order for a given device and shape).  The row statistics
  * are recomputed from q and k.  strides[12]: q row, q head, dq row, dq head,
  * dq_out row, dq_out head, then the same of k.  A token whose position is
@@ -522,7 +522,7 @@ int bokt_moe_combine(const void* y, int64_t y_rows, const int32_t* rows, const f
  * with [Wg | Wu] = w_gate_up[e] ([K, 2 I]) and Wd = w_down[e] ([I, K]).  The
  * weights of every expert in use are read once.  silu(gate) * up is rounded to
  * dtype (it is a tensor-core operand); the experts' results are summed in fp32
- * and rounded once.  x, out [tokens, K]; logits [tokens, E] fp16/bf16/fp32.
+ * and rounded once.  x, out [tokens, K] (out may be x); logits [tokens, E] fp16/bf16/fp32.
  * A NaN logit makes its token's gates and output NaN.  tokens <= 128,
  * topk <= 8, E <= 1024, K and I multiples of 8, 16-byte aligned pointers (else
  * BOKT_ERR_UNSUPPORTED: larger batches go through bokt_moe_topk_gate,
@@ -555,7 +555,9 @@ int bokt_kernel_attrs(int kernel, int dtype, int n, int k, const bokt_params* pa
 
 /*
  * Device status word of the current device: 0 when no kernel has reported a
- * bounded-wait timeout or an out-of-range routing id since the last reset.
+ * bounded-wait timeout (1), an out-of-range routing id (2), a plan mismatch (3)
+ * or overflow (4), a position outside its table (5) or a bad adapter id (6)
+ * since the last reset; detail: where, or which row.
  * Synchronises the device.  reset != 0 clears it.
  */
 int bokt_device_status(int* code, int* detail, int reset);

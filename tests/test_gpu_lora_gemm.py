@@ -182,6 +182,12 @@ def test_unaligned_tensors_are_refused(cuda_device):
         lora_gemm.launch(c.x, c.w, c.bank, c.ids, flat[1:].view(4, 128))
 
 
+def test_output_over_the_input_is_refused(cuda_device):
+    c = Case(4, 64, 64, 3, 16)
+    with pytest.raises(ValueError, match="overlap"):
+        lora_gemm.launch(c.x, c.w, c.bank, c.ids, c.x)
+
+
 def test_adapter_changed_between_calls(cuda_device):
     c = Case(30, 64, 128, 4, 16)
     c.run()

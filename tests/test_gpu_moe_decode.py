@@ -171,6 +171,14 @@ def test_weights_that_are_not_finite_reach_their_tokens_only(t, cuda_device):
     assert hit.any() and torch.isnan(out[hit]).all() and torch.equal(out[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("t", [3, 50])
+def test_output_over_the_input(t, cuda_device):
+    a = make(t, 8, 264, 136)
+    want = run(a, 2)
+    moe_decode.launch(**a, out=a["x"], topk=2)
+    assert torch.equal(a["x"], want)
+
+
 def test_no_tokens(cuda_device):
     a = make(0, 4, 64, 32)
     assert run(a, 2).shape == (0, 64)

@@ -88,6 +88,16 @@ def test_launch_refusals(over, match):
         call(**over)
 
 
+def test_bank_loads_what_other_memory_holds():
+    """Strided and transposed adapters are copied, not referenced."""
+    b = bank()
+    a1, b1 = torch.randn(16, 8).to(BF), torch.randn(8, 48).to(BF)
+    b.load(1, a1.t(), b1[:, ::2], 2.0)
+    want = a1.t().clone()
+    a1.zero_()
+    assert torch.equal(b.a[1, :8], want) and torch.equal(b.b[1, :8], b1[:, ::2])
+
+
 def test_c_abi_argument_errors_need_no_gpu():
     lib = _native.load()
 

@@ -81,3 +81,9 @@ def test_c_abi_argument_errors_need_no_gpu():
     assert lib.bokt_qk_norm_rope(*args(eps=float("nan"))) == 1
     assert lib.bokt_rope_table(None, 4, 3, 10000.0, None) == 1
     assert lib.bokt_rope_table(None, 0, 4, 10000.0, None) == 0
+
+
+def test_one_buffer_for_both_weight_gradients_is_refused():
+    both = torch.zeros(16)
+    with pytest.raises(ValueError, match="separate"):
+        call(backward=True, dq_weight=both, dk_weight=both)
