@@ -5,7 +5,6 @@ fallback behind the ``launch`` functions.  A missing or stale library raises
 ``RuntimeError`` at the first call instead of silently running something else.
 """
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -194,38 +193,28 @@ def make_params(params):
     return p
 
 
-def dtype_code(dtype):
-    import torch
+_dtype_codes = {}
 
-    if dtype == torch.bfloat16:
-        return BF16
-    if dtype == torch.float16:
-        return FP16
-    raise ValueError(f"Unsupported dtype {dtype}; expected float16 or bfloat16")
+
+def dtype_code(dtype):
+    code = _dtype_codes.get(dtype)
+    if code is None:
+        import torch
+
+        _dtype_codes.update({torch.bfloat16: BF16, torch.float16: FP16})
+        code = _dtype_codes.get(dtype)
+        if code is None:
+            raise ValueError(f"Unsupported dtype {dtype}; expected float16 or bfloat16")
+    return code
 
 
 def current_stream(device):
-    """Handle of torch's current stream on a device (or device index), without
-    building the Stream object, which costs more than a decode kernel runs."""
+    """Handle of torch's current stream on a device, without building the Stream
+    object, which costs more than a decode kernel runs."""
     import torch
 
-    index = device if isinstance(device, int) else device.index
-    if index is None:
-        index = torch.cuda.current_device()
+    index = torch.cuda.current_device() if device.index is None else device.index
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index))
-
-
-_SAME_DEVICE = contextlib.nullcontext()
-
-
-def on_device(index):
-    """Context in which device ``index`` (a tensor's) is the current CUDA device;
-    the library launches on the current one.  Free of cost where it already is."""
-    import torch
-
-    if torch._C._cuda_getDevice() == index:
-        return _SAME_DEVICE
-    return torch.cuda.device(index)
 
 
 _workspace_need = {}
@@ -240,20 +229,21 @@ def workspace(entry, sizes, index, given):
     import torch
 
     key = (entry, sizes, index)
-    need = _workspace_need.get(key)
-    if need is None:
+    known = _workspace_need.get(key)
+    if known is None:
         lib = load()
         need = int(getattr(lib, entry)(*sizes))
         if need < 0:
             raise RuntimeError(f"{entry}: {lib.bokt_last_error().decode(errors='replace')}")
         if len(_workspace_need) >= 4096:
             _workspace_need.clear()
-        _workspace_need[key] = need
+        known = _workspace_need[key] = (need, torch.device("cuda", index))
+    need, device = known
     if given is None:
-        return torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index)), need
+        return torch.empty(need, dtype=torch.uint8, device=device), need
     have = given.numel() * given.element_size()
     if given.get_device() != index or not given.is_contiguous() or have < need:
-        raise ValueError(f"workspace must be a contiguous tensor of {need} bytes on cuda:{index}")
+        raise ValueError(f"workspace must be a contiguous tensor of {need} bytes on {device}")
     return given, have
 
 

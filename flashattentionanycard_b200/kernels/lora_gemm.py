@@ -124,13 +124,15 @@ def launch(x, w, bank, ids, out, workspace=None):
     xp, outp = x.data_ptr(), out.data_ptr()
     if xp < outp + 2 * m * n and outp < xp + 2 * m * k:
         raise ValueError("out must not overlap x: finished columns are written while others still read x")
-    lib = _native.load()
-    with _native.on_device(index):
-        scratch, nbytes = _native.workspace("bokt_lora_gemm_workspace_bytes", (m, n, k, bank.slots, bank.rank),
-                                            index, workspace)
-        rc = lib.bokt_lora_gemm(
-            xp, w.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
-            bank.ranks.data_ptr(), ids.data_ptr(), outp, m, n, k, bank.slots, bank.rank,
-            _native.dtype_code(dtype), scratch.data_ptr(), nbytes, _native.current_stream(index))
-    _native.check(rc, "bokt_lora_gemm")
+    if torch._C._cuda_getDevice() != index:  # the library launches on the current device
+        with torch.cuda.device(index):
+            return launch(x, w, bank, ids, out, workspace)
+    scratch, nbytes = _native.workspace("bokt_lora_gemm_workspace_bytes", (m, n, k, bank.slots, bank.rank),
+                                        index, workspace)
+    rc = _native.load().bokt_lora_gemm(
+        xp, w.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), bank.scales.data_ptr(),
+        bank.ranks.data_ptr(), ids.data_ptr(), outp, m, n, k, bank.slots, bank.rank,
+        _native.dtype_code(dtype), scratch.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _native.check(rc, "bokt_lora_gemm")
     return out

@@ -68,13 +68,15 @@ def launch(x, logits, w_gate_up, w_down, out, topk, renormalize=True, workspace=
     if index < 0 or not (logits.get_device() == w_gate_up.get_device() == w_down.get_device()
                          == out.get_device() == index):
         raise ValueError("all tensors must be on one CUDA device")
-    lib = _native.load()
-    with _native.on_device(index):
-        scratch, nbytes = _native.workspace("bokt_moe_decode_workspace_bytes", (t, e, k, inner, topk), index,
-                                            workspace)
-        rc = lib.bokt_moe_decode(
-            x.data_ptr(), logits.data_ptr(), logits_dtype, w_gate_up.data_ptr(), w_down.data_ptr(),
-            out.data_ptr(), t, e, k, inner, topk, 1 if renormalize else 0, dtype, scratch.data_ptr(), nbytes,
-            _native.current_stream(index))
-    _native.check(rc, "bokt_moe_decode")
+    if torch._C._cuda_getDevice() != index:  # the library launches on the current device
+        with torch.cuda.device(index):
+            return launch(x, logits, w_gate_up, w_down, out, topk, renormalize, workspace)
+    scratch, nbytes = _native.workspace("bokt_moe_decode_workspace_bytes", (t, e, k, inner, topk), index,
+                                        workspace)
+    rc = _native.load().bokt_moe_decode(
+        x.data_ptr(), logits.data_ptr(), logits_dtype, w_gate_up.data_ptr(), w_down.data_ptr(),
+        out.data_ptr(), t, e, k, inner, topk, 1 if renormalize else 0, dtype, scratch.data_ptr(), nbytes,
+        torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _native.check(rc, "bokt_moe_decode")
     return out

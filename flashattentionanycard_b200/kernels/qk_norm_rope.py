@@ -18,8 +18,8 @@ The rotation turns the pairs (i, i + rot / 2), or with ``interleaved`` the
 neighbours (2 i, 2 i + 1).
 """
 
-import ctypes
 import math
+import struct
 
 from flashattentionanycard_b200 import _native
 
@@ -34,7 +34,7 @@ def rope_table(rows, rot, base=10000.0, device="cuda"):
     if not (math.isfinite(base) and base > 0):
         raise ValueError("base must be finite and positive")
     out = torch.empty((rows, rot), device=device, dtype=torch.float32)
-    with _native.on_device(out.get_device()):
+    with torch.cuda.device(out.device):
         _native.check(
             _native.load().bokt_rope_table(out.data_ptr(), rows, rot, float(base),
                                            _native.current_stream(out.device)),
@@ -45,7 +45,7 @@ def rope_table(rows, rot, base=10000.0, device="cuda"):
 
 # Decode calls are shorter than their checks: each check below is a plain
 # comparison, and every attribute is read once.
-_Strides = ctypes.c_int64 * 12
+_pack8, _pack12 = struct.Struct("8q").pack, struct.Struct("12q").pack  # int64 strides
 
 
 def _views(named, shape, dtype, index):
@@ -113,19 +113,24 @@ def _check(q, k, q_weight, k_weight, positions, cos_sin, epsilon):
 
 def launch(q, k, q_weight, k_weight, positions, cos_sin, q_out, k_out, epsilon=1e-6, interleaved=False):
     """q_out, k_out = rotated norms of q's and k's heads (q_out may be q, k_out may be k)."""
+    import torch
+
     qs, ks, rot, rows, index, i64 = _check(q, k, q_weight, k_weight, positions, cos_sin, epsilon)
     dtype = q.dtype
-    strides = _Strides(*_views((("q", q, False), ("q_out", q_out, True)), qs, dtype, index),
-                       *_views((("k", k, False), ("k_out", k_out, True)), ks, dtype, index))
+    strides = _pack8(*_views((("q", q, False), ("q_out", q_out, True)), qs, dtype, index),
+                     *_views((("k", k, False), ("k_out", k_out, True)), ks, dtype, index))
     if index < 0:
         raise ValueError("q, k and their tensors must be CUDA tensors")
-    lib = _native.load()
-    with _native.on_device(index):
-        rc = lib.bokt_qk_norm_rope(
-            q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), i64,
-            cos_sin.data_ptr(), rows, q_out.data_ptr(), k_out.data_ptr(), qs[0], qs[1], ks[1], qs[2], rot,
-            strides, 1 if interleaved else 0, epsilon, _native.dtype_code(dtype), _native.current_stream(index))
-    _native.check(rc, "bokt_qk_norm_rope")
+    if torch._C._cuda_getDevice() != index:  # the library launches on the current device
+        with torch.cuda.device(index):
+            return launch(q, k, q_weight, k_weight, positions, cos_sin, q_out, k_out, epsilon, interleaved)
+    rc = _native.load().bokt_qk_norm_rope(
+        q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), i64,
+        cos_sin.data_ptr(), rows, q_out.data_ptr(), k_out.data_ptr(), qs[0], qs[1], ks[1], qs[2], rot,
+        strides, 1 if interleaved else 0, epsilon, _native.dtype_code(dtype),
+        torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _native.check(rc, "bokt_qk_norm_rope")
     return q_out, k_out
 
 
@@ -138,7 +143,7 @@ def launch_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, cos_sin
 
     qs, ks, rot, rows, index, i64 = _check(q, k, q_weight, k_weight, positions, cos_sin, epsilon)
     dtype, d = q.dtype, qs[2]
-    strides = _Strides(
+    strides = _pack12(
         *_views((("q", q, False), ("dq", dq, True), ("dq_out", dq_out, False)), qs, dtype, index),
         *_views((("k", k, False), ("dk", dk, True), ("dk_out", dk_out, False)), ks, dtype, index))
     _weight("dq_weight", dq_weight, d, torch.float32, index)
@@ -147,14 +152,17 @@ def launch_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, cos_sin
         raise ValueError("dq_weight and dk_weight must be separate buffers (add them where q and k share a weight)")
     if index < 0:
         raise ValueError("q, k and their tensors must be CUDA tensors")
-    lib = _native.load()
-    with _native.on_device(index):
-        scratch, nbytes = _native.workspace("bokt_qk_norm_rope_workspace_bytes", (d,), index, None)
-        rc = lib.bokt_qk_norm_rope_backward(
-            dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(), q_weight.data_ptr(),
-            k_weight.data_ptr(), positions.data_ptr(), i64, cos_sin.data_ptr(), rows, dq.data_ptr(),
-            dk.data_ptr(), dq_weight.data_ptr(), dk_weight.data_ptr(), qs[0], qs[1], ks[1], d, rot, strides,
-            1 if interleaved else 0, epsilon, _native.dtype_code(dtype), scratch.data_ptr(), nbytes,
-            _native.current_stream(index))
-    _native.check(rc, "bokt_qk_norm_rope_backward")
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return launch_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, cos_sin, dq, dk,
+                                   dq_weight, dk_weight, epsilon, interleaved)
+    scratch, nbytes = _native.workspace("bokt_qk_norm_rope_workspace_bytes", (d,), index, None)
+    rc = _native.load().bokt_qk_norm_rope_backward(
+        dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(), q_weight.data_ptr(),
+        k_weight.data_ptr(), positions.data_ptr(), i64, cos_sin.data_ptr(), rows, dq.data_ptr(),
+        dk.data_ptr(), dq_weight.data_ptr(), dk_weight.data_ptr(), qs[0], qs[1], ks[1], d, rot, strides,
+        1 if interleaved else 0, epsilon, _native.dtype_code(dtype), scratch.data_ptr(), nbytes,
+        torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _native.check(rc, "bokt_qk_norm_rope_backward")
     return dq, dk, dq_weight, dk_weight
