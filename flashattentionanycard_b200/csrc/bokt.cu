@@ -1532,7 +1532,7 @@ cudaError_t launch_qk_vec(bokt::QkArgs a, int sm_count, int* blocks, cudaStream_
   const long long u0 = (long long)a.tokens * ((a.side[0].heads + hpu - 1) / hpu);
   const long long u1 = (long long)a.tokens * ((a.side[1].heads + hpu - 1) / hpu);
   if constexpr (GRAD) {
-    long long grid = ((u0 > u1 ? u0 : u1) + bokt::kQkWarps - 1) / bokt::kQkWarps;
+    long long grid = (u0 + u1 + bokt::kQkWarps - 1) / bokt::kQkWarps;
     if (grid > (long long)kQkGradBlocksPerSm * sm_count)
       grid = (long long)kQkGradBlocksPerSm * sm_count;
     *blocks = int(grid);

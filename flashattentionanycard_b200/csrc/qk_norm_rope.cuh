@@ -248,15 +248,19 @@ __device__ __forceinline__ void qk_copy_async(uint4* dst, const void* src, bool 
                : "memory");
 }
 
-// Rows of one warp's walk: batches of R heads per lane group, unit after unit.
+// Rows of one warp's walk over the units of both sides (a token's query units,
+// then its key units): batches of R heads per lane group, unit after unit.
 struct QkWalk {
-  int u, t, h0, hend;
-  __device__ __forceinline__ void enter(int unit, int chunks, int hpu, int heads, int sub) {
+  int u, t, h0, hend, side;
+  __device__ __forceinline__ void enter(const QkArgs& args, int unit, int chunks0, int chunks, int hpu,
+                                        int sub) {
     u = unit;
     t = unit / chunks;
-    const int chunk = unit - t * chunks;
+    int chunk = unit - t * chunks;
+    side = chunk >= chunks0;
+    if (side) chunk -= chunks0;
     h0 = chunk * hpu + sub;
-    hend = min(heads, (chunk + 1) * hpu);
+    hend = min(args.side[side].heads, (chunk + 1) * hpu);
   }
 };
 
@@ -271,11 +275,11 @@ __host__ __device__ constexpr int qk_grad_smem_bytes() {
   return ring > sums ? ring : sums;
 }
 
-// Backward: persistent warps walk the query units, then the key units.  The
-// next batches' rows arrive by cp.async while one is computed (each lane reads
-// back what it copied itself: no barrier); the weight gradient of a side stays
-// in 8 registers per lane until its last unit, is summed over the block's rows
-// in shared memory and leaves as one partial row per block, which
+// Backward: persistent warps walk the units of all tokens.  The next batches'
+// rows arrive by cp.async while one is computed (each lane reads back what it
+// copied itself: no barrier); the weight gradients stay in 8 registers a side
+// and lane until the end, are summed over the block's rows in shared memory and
+// leave as one partial row per block and side, which
 // qk_norm_rope_dweight_kernel adds in block order.
 template <typename T, int L, bool PAIRS, int R>
 __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const QkArgs args) {
@@ -291,99 +295,111 @@ __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const 
   const int partner = PAIRS || !turns ? lane : (i < args.rot / 2 ? lane + half : lane - half);
   uint4* ring = qk_ring + threadIdx.x;  // [slot][row][x, gradient][thread]
   const int stride = gridDim.x * kQkWarps;
+  const int hpu = S * R * args.loops;
+  const int chunks0 = (args.side[0].heads + hpu - 1) / hpu;
+  const int chunks = chunks0 + (args.side[1].heads + hpu - 1) / hpu;
+  const int units = args.tokens * chunks;
   pdl_wait();
-#pragma unroll 1
-  for (int side = 0; side < 2; ++side) {
-    const QkSide& sd = args.side[side];
-    const int hpu = S * R * args.loops;
-    const int chunks = (sd.heads + hpu - 1) / hpu;
-    const int units = args.tokens * chunks;
-    float2 w[4], dw[4] = {};
-    qk_unpack<T>(active && units > 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(sd.w) + i)
-                                     : make_uint4(0, 0, 0, 0), w);
-    QkWalk in = {}, at = {};  // the batch to copy next, the batch to compute
-    in.u = at.u = blockIdx.x * kQkWarps + warp;
-    if (in.u < units) in.enter(in.u, chunks, hpu, sd.heads, sub);
-    int slot_in = 0, slot = 0;
-    auto copy = [&] {
-      if (in.u < units) {
-        const T* x = static_cast<const T*>(sd.x) + in.t * sd.x_row + i;
-        const T* g = static_cast<const T*>(sd.g) + in.t * sd.g_row + i;
+  float2 dwq[4] = {}, dwk[4] = {};
+  QkWalk in = {}, at = {};  // the batch to copy next, the batch to compute
+  in.u = at.u = blockIdx.x * kQkWarps + warp;
+  if (in.u < units) in.enter(args, in.u, chunks0, chunks, hpu, sub);
+  int slot_in = 0, slot = 0;
+  auto copy = [&] {
+    if (in.u < units) {
+      const QkSide& sd = args.side[in.side];
+      const T* x = static_cast<const T*>(sd.x) + in.t * sd.x_row + i;
+      const T* g = static_cast<const T*>(sd.g) + in.t * sd.g_row + i;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int h = in.h0 + r * S;
-          const bool have = active && h < in.hend;
-          uint4* dst = ring + (slot_in * R + r) * 2 * kQkThreads;
-          qk_copy_async(dst, have ? x + h * sd.x_head : sd.x, have);
-          qk_copy_async(dst + kQkThreads, have ? g + h * sd.g_head : sd.g, have);
-        }
-        slot_in = slot_in + 1 == kQkRing ? 0 : slot_in + 1;
-        in.h0 += S * R;
-        if (in.h0 - sub >= in.hend) {
-          in.u += stride;
-          if (in.u < units) in.enter(in.u, chunks, hpu, sd.heads, sub);
-        }
+      for (int r = 0; r < R; ++r) {
+        const int h = in.h0 + r * S;
+        const bool have = active && h < in.hend;
+        uint4* dst = ring + (slot_in * R + r) * 2 * kQkThreads;
+        qk_copy_async(dst, have ? x + h * sd.x_head : sd.x, have);
+        qk_copy_async(dst + kQkThreads, have ? g + h * sd.g_head : sd.g, have);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    for (int s = 0; s < kQkRing - 1; ++s) copy();
-    long long next = at.u < units ? qk_position(args, at.u / chunks) : 0;
-#pragma unroll 1
-    for (; at.u < units; at.u += stride) {
-      at.enter(at.u, chunks, hpu, sd.heads, sub);
-      const long long pos = next;
-      if (at.u + stride < units) next = qk_position(args, (at.u + stride) / chunks);
-      const bool known = pos >= 0 && pos < args.table_rows;
-      if (!known && lane == 0) report_status(kStatusBadPosition, at.t);
-      QkAngles ang;
-      if (turns && known) {
-        qk_load_angles<PAIRS>(args.cos_sin + pos * args.rot, args.rot, i, ang);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ang.s[j] = make_float2(-ang.s[j].x, -ang.s[j].y);  // backwards
-      }
-      T* out = static_cast<T*>(sd.out) + at.t * sd.out_row + i;
-#pragma unroll 1
-      for (; at.h0 - sub < at.hend; at.h0 += S * R) {
-        copy();
-        asm volatile("cp.async.wait_group %0;" ::"n"(kQkRing - 1) : "memory");
-        const uint4* row = ring + slot * R * 2 * kQkThreads;
-        slot = slot + 1 == kQkRing ? 0 : slot + 1;
-        if (!known) continue;  // its rows stay unwritten and add nothing
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int h = at.h0 + r * S;
-          const uint4 xr = row[r * 2 * kQkThreads], gr = row[(r * 2 + 1) * kQkThreads];
-          float2 v[4], gv[4], o[4], ss = both(0.f), dot = both(0.f);
-          qk_unpack<T>(xr, v);
-          qk_unpack<T>(gr, gv);
-          qk_partner<T, PAIRS>(gr, gv, partner, o);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            gv[j] = fma2(gv[j], ang.c[j], mul2(o[j], ang.s[j]));  // turned back
-            o[j] = mul2(gv[j], v[j]);
-            gv[j] = mul2(gv[j], w[j]);
-            ss = fma2(v[j], v[j], ss);
-            dot = fma2(gv[j], v[j], dot);
-          }
-          // Both sums at once; with n = x r: mean(g w n) = r dot / D.
-          const float r1 = rsqrtf(fmaf(qk_row_sum<L>(ss.x + ss.y), inv_dim, args.eps));
-          const float2 rs = both(r1), mean = both(-r1 * inv_dim * qk_row_sum<L>(dot.x + dot.y));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            dw[j] = fma2(o[j], rs, dw[j]);
-            gv[j] = mul2(fma2(mul2(v[j], rs), mean, gv[j]), rs);
-          }
-          if (active && h < at.hend) *reinterpret_cast<uint4*>(out + h * sd.out_head) = qk_pack<T>(gv);
-        }
+      slot_in = slot_in + 1 == kQkRing ? 0 : slot_in + 1;
+      in.h0 += S * R;
+      if (in.h0 - sub >= in.hend) {
+        in.u += stride;
+        if (in.u < units) in.enter(args, in.u, chunks0, chunks, hpu, sub);
       }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();  // the ring turns into the sums
-    float* sums = reinterpret_cast<float*>(qk_ring);
-    constexpr int kRow = L * 8 + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int s = 0; s < kQkRing - 1; ++s) copy();
+  long long next = at.u < units ? qk_position(args, at.u / chunks) : 0;
+#pragma unroll 1
+  for (; at.u < units; at.u += stride) {
+    at.enter(args, at.u, chunks0, chunks, hpu, sub);
+    const QkSide& sd = args.side[at.side];
+    const long long pos = next;
+    if (at.u + stride < units) next = qk_position(args, (at.u + stride) / chunks);
+    const bool known = pos >= 0 && pos < args.table_rows;
+    if (!known && lane == 0) report_status(kStatusBadPosition, at.t);
+    QkAngles ang;
+    if (turns && known) {
+      qk_load_angles<PAIRS>(args.cos_sin + pos * args.rot, args.rot, i, ang);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      sums[(warp * S + sub) * kRow + i + j] = j & 1 ? dw[j / 2].y : dw[j / 2].x;
+      for (int j = 0; j < 4; ++j) ang.s[j] = make_float2(-ang.s[j].x, -ang.s[j].y);  // backwards
+    }
+    const uint4 wraw = active ? *reinterpret_cast<const uint4*>(static_cast<const T*>(sd.w) + i)
+                              : make_uint4(0, 0, 0, 0);
+    T* out = static_cast<T*>(sd.out) + at.t * sd.out_row + i;
+#pragma unroll 1
+    for (; at.h0 - sub < at.hend; at.h0 += S * R) {
+      copy();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kQkRing - 1) : "memory");
+      const uint4* row = ring + slot * R * 2 * kQkThreads;
+      slot = slot + 1 == kQkRing ? 0 : slot + 1;
+      if (!known) continue;  // its rows stay unwritten and add nothing
+      float2 dw[4] = {};
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int h = at.h0 + r * S;
+        const uint4 xr = row[r * 2 * kQkThreads], gr = row[(r * 2 + 1) * kQkThreads];
+        float2 v[4], gv[4], o[4], w[4], ss = both(0.f), dot = both(0.f);
+        qk_unpack<T>(xr, v);
+        qk_unpack<T>(gr, gv);
+        qk_unpack<T>(wraw, w);
+        qk_partner<T, PAIRS>(gr, gv, partner, o);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          gv[j] = fma2(gv[j], ang.c[j], mul2(o[j], ang.s[j]));  // turned back
+          o[j] = mul2(gv[j], v[j]);
+          gv[j] = mul2(gv[j], w[j]);
+          ss = fma2(v[j], v[j], ss);
+          dot = fma2(gv[j], v[j], dot);
+        }
+        // Both sums at once; with n = x r: mean(g w n) = r dot / D.
+        const float r1 = rsqrtf(fmaf(qk_row_sum<L>(ss.x + ss.y), inv_dim, args.eps));
+        const float2 rs = both(r1), mean = both(-r1 * inv_dim * qk_row_sum<L>(dot.x + dot.y));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          dw[j] = fma2(o[j], rs, dw[j]);
+          gv[j] = mul2(fma2(mul2(v[j], rs), mean, gv[j]), rs);
+        }
+        if (active && h < at.hend) *reinterpret_cast<uint4*>(out + h * sd.out_head) = qk_pack<T>(gv);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float2& to = at.side ? dwk[j] : dwq[j];
+        to.x += dw[j].x;
+        to.y += dw[j].y;
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();  // the ring turns into the sums
+  float* sums = reinterpret_cast<float*>(qk_ring);
+  constexpr int kRow = L * 8 + 1;
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 d = side ? dwk[j / 2] : dwq[j / 2];
+      sums[(warp * S + sub) * kRow + i + j] = j & 1 ? d.y : d.x;
+    }
     __syncthreads();
     for (int d = threadIdx.x; d < args.dim; d += kQkThreads) {
       float total = 0.f;
