@@ -153,3 +153,40 @@ def test_training_pair_of_norm_and_rotation(cuda_device):
     size = (np.abs(f64(dout)) + np.abs(f64(q_out)) * 2.0**-8).max() * np.abs(way).sum()
     assert abs(terms.sum() - slope) <= 2.0**-7 * size
     assert not dk.any() and not dw[1].any()
+
+
+def test_operators_of_several_streams_at_once(cuda_device):
+    """Persistent, clustered and small kernels of five streams share the SMs;
+    every result keeps its bits."""
+    from tests import test_gpu_moe_decode as moe
+
+    cases = []
+    for t, e, k, inner, topk in ((1, 8, 512, 1024, 2), (12, 16, 264, 520, 3), (90, 30, 256, 768, 5), (128, 64, 512, 256, 8)):
+        a = moe.make(t, e, k, inner, seed=t)
+        cases.append(lambda a=a, topk=topk: moe.run(a, topk))
+    for t in (5, 200, 900):
+        c = Case(t, 512, 1032, 9, 24, seed=t)
+        cases.append(c.run)
+    layer = Layer(60)
+    a, b = torch.randn(300, 512, device="cuda").to(BF), torch.randn(512, 264, device="cuda").to(BF)
+    odd = torch.randn(37, 77, device="cuda").to(BF), torch.randn(77, 93, device="cuda").to(BF)
+
+    def product(x, w):
+        out = torch.empty(x.shape[0], w.shape[1], dtype=BF, device="cuda")
+        gemm.launch(x, w, out, {})
+        return out
+
+    cases += [lambda: product(a, b), lambda: product(*odd)]
+    layer.step()
+    want = [c() for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(5)]
+    got = []
+    for turn in range(6):
+        for i, c in enumerate(cases):
+            s = streams[(i + turn) % len(streams)]
+            with torch.cuda.stream(s):
+                got.append((i, c()))
+    torch.cuda.synchronize()
+    for i, out in got:
+        assert torch.equal(out, want[i]), i

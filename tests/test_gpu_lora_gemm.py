@@ -89,6 +89,9 @@ SHAPES = [
     (200, 128, 4096, 33, 32, 20), (256, 328, 200, 1000, 16, None), (257, 64, 64, 2, 16, None),
     (300, 1000, 520, 300, 16, None), (1000, 256, 1000, 9, 128, 11), (2100, 200, 776, 30, 33, 40),
     (5000, 72, 256, 4, 64, 3), (63, 2048, 20000, 6, 16, None), (1500, 8, 8, 3, 8, 2),
+    # the longest lists: every row of a tile its own adapter
+    (256, 72, 264, 1024, 128, None), (520, 136, 72, 1024, 128, None), (700, 64, 520, 700, 64, None),
+    (128, 256, 20000, 500, 32, None),
 ]
 
 

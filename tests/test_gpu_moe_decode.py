@@ -93,6 +93,8 @@ SHAPES = [
     # sixteen tokens and fewer on either kernel: more assignments, long runs, wide outputs
     (9, 64, 128, 72, 8), (16, 64, 256, 1024, 4), (16, 3, 2056, 136, 2), (8, 40, 4104, 24, 8),
     (13, 600, 264, 40, 4), (2, 2, 20000, 16, 2),
+    # the largest lists
+    (128, 1024, 8, 8, 8), (128, 1024, 72, 136, 8), (128, 8, 264, 72, 8), (16, 4, 264, 2056, 4),
 ]
 
 
