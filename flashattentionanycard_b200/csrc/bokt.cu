@@ -1925,13 +1925,13 @@ int bokt_moe_decode(const void* x, const void* logits, int logits_dtype, const v
 // ----------------------------------------------------------------- projection with adapters
 namespace {
 
-// Rows up to which the weight-streaming kernel is used.
-constexpr int kLoraStreamRows = 256;
+// Rows up to which W is always streamed, beside the shrink of few rows.
+constexpr int kLoraFewRows = 256;
 // Shared memory left to a shrink CTA (rank 16: 9 KB of partials, 7 KB of lists).
 constexpr int kLoraShrinkSmem = 20 * 1024;
 
 struct LoraPlan {
-  bool stream;
+  bool stream, shrink_tc;
   int tile_rows, tiles, smax, gmax, cluster, stages;
   int shrink_cluster, walkers;
   int64_t count, list, h, total;
@@ -1978,7 +1978,14 @@ int lora_plan(int M, int N, int K, int slots, int rank, const DeviceInfo& dev, L
   if (K % 8 != 0 || N % 8 != 0)
     return fail(BOKT_ERR_UNSUPPORTED, "K and N must be multiples of 8 (got %d, %d)", K, N);
   *p = {};
-  p->stream = M <= kLoraStreamRows;
+  // Few rows stream W; so do more of them while the 128 x 128 tiles leave SMs to
+  // split K over (1024 x 1024 of K = 4096: 21 us, 26 on pair tiles; 4096 wide: 35
+  // on pair tiles, 82 streamed).  The shrink of many rows is faster from 257 on
+  // with a few adapters a row tile (512 rows of 9: 27 and 34 us), and slower up to
+  // 700 rows with many (512 rows of 16 adapters of rank 64: 59 and 41).
+  const long long small_tiles = (long long)((M + 127) / 128) * ((N + 127) / 128);
+  p->stream = M <= kLoraFewRows || small_tiles * 2 <= dev.sm_count;
+  p->shrink_tc = M > kLoraFewRows;
   if (p->stream) {
     const int chunks = (M + 127) / 128;
     p->tiles = chunks;
@@ -2117,7 +2124,7 @@ int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void*
     if ((rc = encode_map(&mb, lora_b, 3, d, st, b, fp16))) return rc;
   }
   cudaError_t e;
-  if (p.stream) {
+  if (!p.shrink_tc) {
     int smem = 0;
     const void* fn = fp16 ? lora_shrink_ptr<__half>(rank, &smem) : lora_shrink_ptr<__nv_bfloat16>(rank, &smem);
     if ((rc = ensure_smem(fn, smem)) || (rc = ensure_carveout(fn))) return rc;
@@ -2133,11 +2140,13 @@ int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void*
     if ((rc = encode_map(&ma, lora_a, 2, d, st, b, fp16))) return rc;
     a.idesc = bokt::make_idesc_f16_kk(uint32_t(dtype), 0);
     a.stages = 5;
-    const int smem = bokt::lora_shrink_tc_smem_bytes(a.stages);
+    while (a.stages > 2 && bokt::lora_shrink_tc_smem_bytes(a.stages, rank) + 8192 > dev.smem_optin) --a.stages;
+    const int smem = bokt::lora_shrink_tc_smem_bytes(a.stages, rank);
     const void* fn = fp16 ? reinterpret_cast<const void*>(&bokt::lora_shrink_tc_kernel<__half>)
                           : reinterpret_cast<const void*>(&bokt::lora_shrink_tc_kernel<__nv_bfloat16>);
     if ((rc = ensure_smem(fn, smem))) return rc;
-    const int clusters = (M + bokt::kLoraShrinkRows - 1) / bokt::kLoraShrinkRows;
+    a.shrink_rows = p.tile_rows < bokt::kLoraShrinkRows ? p.tile_rows : bokt::kLoraShrinkRows;
+    const int clusters = (M + a.shrink_rows - 1) / a.shrink_rows;
     void* kargs[] = {&mx, &ma, &a};
     e = launch_cluster(fn, clusters * bokt::kLoraShrinkSplit, bokt::kLoraThreads, smem,
                        bokt::kLoraShrinkSplit, s, kargs);

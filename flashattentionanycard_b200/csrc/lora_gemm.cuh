@@ -17,9 +17,10 @@
 //       would idle on an adapter's handful of tokens).
 //   lora_shrink_tc_kernel  the same for many tokens: bound by reading x; 128
 //       tokens a cluster of four CTAs that split K, TMA ring and tcgen05.
-//   lora_stream_kernel  few tokens (row tiles of up to 128): bound by reading W.
-//       W tiles are the 128-row operand and the tokens the narrow one; a cluster
-//       of C CTAs splits K and reduces through distributed shared memory.
+//   lora_stream_kernel  few tokens, or few tiles (row tiles of up to 128): bound
+//       by reading W.  W tiles are the 128-row operand and the tokens the narrow
+//       one; a cluster of C CTAs splits K and reduces through distributed shared
+//       memory.
 //   lora_tc2_kernel     many tokens: the CTA-pair GEMM's 256 x 256 tiles.
 // Both products start on x and W while the shrink kernel still runs: it lets
 // its dependents go only after its own wait, so everything before it is
@@ -53,6 +54,7 @@ struct LoraArgs {
   int walkers;            // shrink: clusters per row tile, each walking every walkers-th entry
   int cluster;            // CTAs per cluster of the kernel at hand
   int stages, group_m, chunks;
+  int shrink_rows;        // lora_shrink_tc_kernel: tokens per cluster (at most 128, whole in a row tile)
   uint32_t idesc;
 };
 
@@ -286,18 +288,18 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
 constexpr int kLoraShrinkRows = 128, kLoraShrinkSplit = 4;  // tokens and CTAs of a cluster
 constexpr int kLoraShrinkCols = 128;                        // accumulator columns of a pass
 constexpr int kLoraShrinkStage = (kLoraShrinkRows + kLoraShrinkCols) * 128;
-constexpr int kLoraShrinkRecv = kLoraShrinkSplit * 32 * 64 * 4;
 
-__host__ __device__ inline int lora_shrink_tc_smem_bytes(int stages) {
-  return 1024 + stages * kLoraShrinkStage + kLoraShrinkRecv + (2 * stages + 2) * 8 + 16;
+__host__ __device__ inline int lora_shrink_tc_smem_bytes(int stages, int rank) {
+  return 1024 + stages * kLoraShrinkStage + kLoraShrinkSplit * 32 * rank * 4 + (2 * stages + 4) * 8 + 16;
 }
 
-// H and the lists for row tiles of kLoraPairRows, many tokens.  A cluster takes
-// 128 tokens; CTA r runs a quarter of K: x as the 128-row operand, the A rows of
-// the adapters that these tokens use as the narrow one, 128 columns (128 / R
-// adapters) a pass.  A token keeps the columns of its own adapter; CTA r sums
-// and writes those of tokens [32 r, +32) after the quarters have met in its
-// shared memory, in rank order.
+// H and the lists, many tokens.  A cluster takes shrink_rows tokens (a row tile,
+// or half a pair's); CTA r runs a quarter of K: x as the 128-row operand, the A
+// rows of the adapters that these tokens use as the narrow one, 128 columns
+// (128 / R adapters) a pass, two accumulators.  A token keeps the columns of its
+// own adapter, so all passes fill one [tokens][R] buffer in distributed shared
+// memory: CTA r collects the quarters of tokens [32 r, +32), and after one
+// cluster barrier sums them in rank order.
 template <typename T>
 __global__ void __launch_bounds__(kLoraThreads, 1)
     lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tm_x,
@@ -306,22 +308,24 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int stages = args.stages;
-  float* recv = reinterpret_cast<float*>(smem + stages * kLoraShrinkStage);  // [4][32][rs]
-  uint64_t* full = reinterpret_cast<uint64_t*>(recv + kLoraShrinkRecv / 4);
+  const int R = args.rank, rs = min(R, 64);
+  float* recv = reinterpret_cast<float*>(smem + stages * kLoraShrinkStage);  // [4][32][R]
+  uint64_t* full = reinterpret_cast<uint64_t*>(recv + kLoraShrinkSplit * 32 * R);
   uint64_t* empty = full + stages;
   uint64_t* tfull = empty + stages;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tfull + 2);
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   __shared__ int s_flag[kLoraMaxSlots];  // 1 used by the row tile, 3 also by these tokens; then the place
-  __shared__ int s_place[kLoraPairRows];  // of these tokens' adapters: place in the row tile's list
-  __shared__ int s_slot[kLoraPairRows];   // and slot
-  __shared__ int s_id[kLoraShrinkRows], s_warp[8], s_mine[8];
+  __shared__ int s_slot[kLoraShrinkRows];  // the adapters of these tokens
+  __shared__ int s_id[kLoraShrinkRows], s_own[kLoraShrinkRows], s_warp[8], s_mine[8];
+  __shared__ float s_scale[kLoraShrinkRows];
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int rank = static_cast<int>(cluster_ctarank());
-  const int t0 = static_cast<int>(blockIdx.x) / kLoraShrinkSplit * kLoraShrinkRows;
-  const int mt = t0 / kLoraPairRows, m0 = mt * kLoraPairRows;
-  const int R = args.rank, rs = min(R, 64);
+  const int per = args.shrink_rows;
+  const int t0 = static_cast<int>(blockIdx.x) / kLoraShrinkSplit * per;
+  const int mt = t0 / args.tile_rows, m0 = mt * args.tile_rows;
   const int nkb = (args.K + 63) / 64;
   const int kb0 = rank * nkb / kLoraShrinkSplit, kb1 = (rank + 1) * nkb / kLoraShrinkSplit;
 
@@ -330,33 +334,42 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(tfull, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 4);
+    }
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_x);
     tma_prefetch_desc(&tm_a);
   }
   if (warp == 3) {
-    tmem_alloc(tmem_holder, kLoraShrinkCols);
+    tmem_alloc(tmem_holder, 2 * kLoraShrinkCols);
     tmem_relinquish();
   }
   for (int i = tid; i < args.slots; i += kLoraThreads) s_flag[i] = 0;
   cluster_sync();  // every CTA runs before another writes its shared memory
   pdl_wait();
   pdl_allow_next();
-  // Adapters of the row tile (256 rows, one per thread) and of these 128 tokens.
+  // Adapters of the row tile (at most 256 rows, one per thread) and of these tokens.
   int my_id = -1;
-  const bool here = m0 + tid >= t0 && m0 + tid < t0 + kLoraShrinkRows;
-  if (m0 + tid < args.M) {
+  const bool here = m0 + tid >= t0 && m0 + tid < t0 + per;
+  if (tid < args.tile_rows && m0 + tid < args.M) {
     const int id = args.ids[m0 + tid];
-    if (id >= 0 && id < args.slots && args.ranks[id] > 0) {
+    const int own_rank = id >= 0 && id < args.slots ? args.ranks[id] : 0;
+    if (own_rank > 0) {
       my_id = id;
       atomicOr(&s_flag[id], here ? 3 : 1);
+      if (here) {
+        s_own[m0 + tid - t0] = own_rank;
+        s_scale[m0 + tid - t0] = args.scales[id];
+      }
     } else if (id != -1 && here && rank == 0) {
       report_status(kStatusBadAdapter, m0 + tid);
     }
   }
   if (here) s_id[m0 + tid - t0] = my_id;
+  if (tid >= per && tid < kLoraShrinkRows) s_id[tid] = -1;
   __syncthreads();
   int place[4], mine[4], used = 0, own = 0;
 #pragma unroll
@@ -391,33 +404,31 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
     if (place[i] < 0) continue;
     s_flag[slot] = before + place[i];
     if (writes_list) args.list[mt * args.smax + before + place[i]] = slot;
-    if (mine[i] >= 0) {
-      s_place[before_own + mine[i]] = before + place[i];
-      s_slot[before_own + mine[i]] = slot;
-    }
+    if (mine[i] >= 0) s_slot[before_own + mine[i]] = slot;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
 
-  T* h = static_cast<T*>(args.h) + static_cast<size_t>(mt) * args.gmax * kLoraPairRows * 64;
-  const size_t group = static_cast<size_t>(kLoraPairRows) * 64;
+  T* h = static_cast<T*>(args.h) + static_cast<size_t>(mt) * args.gmax * args.tile_rows * 64;
+  const size_t group = static_cast<size_t>(args.tile_rows) * 64;
   const int per_pass = kLoraShrinkCols / R;
-  int stage = 0;
-  uint32_t phase = 0;
-  bool ok = true;
-  for (int p0 = 0, pass = 0; p0 < adapters; p0 += per_pass, ++pass) {
-    const int na = min(per_pass, adapters - p0);
-    if (warp == 0) {
-      if (elect_one()) {
+  const int passes = kb1 > kb0 ? (adapters + per_pass - 1) / per_pass : 0;
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int p = 0; p < passes; ++p) {
+        const int p0 = p * per_pass, cols = min(per_pass, adapters - p0) * R;
         for (int kb = kb0; ok && kb < kb1; ++kb) {
           if (!(ok = mbar_wait(&empty[stage], phase ^ 1u, abort_flag, 71))) break;
           uint8_t* b = smem + stage * kLoraShrinkStage;
-          mbar_arrive_expect_tx(&full[stage], kLoraShrinkRows * 128 + na * R * 128);
+          mbar_arrive_expect_tx(&full[stage], per * 128 + cols * 128);
           tma_load_2d(b, &tm_x, &full[stage], kb * 64, t0);
           b += kLoraShrinkRows * 128;
-          for (int c = 0; c < na * R; c += rs)
+          for (int c = 0; c < cols; c += rs)
             tma_load_2d(b + c * 128, &tm_a, &full[stage], kb * 64, s_slot[p0 + c / R] * R + c % R);
           if (++stage == stages) {
             stage = 0;
@@ -425,9 +436,18 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
           }
         }
       }
-    } else if (warp == 1) {
-      if (elect_one()) {
-        const uint32_t idesc = args.idesc | (static_cast<uint32_t>(na * R >> 3) << 17);
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int p = 0; ok && p < passes; ++p) {
+        const int cols = min(per_pass, adapters - p * per_pass) * R;
+        const uint32_t idesc = args.idesc | (static_cast<uint32_t>(cols >> 3) << 17);
+        if (!(ok = mbar_wait(&tempty[p & 1], (p >> 1 & 1) ^ 1, abort_flag, 74))) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + (p & 1) * kLoraShrinkCols;
         for (int kb = kb0; ok && kb < kb1; ++kb) {
           if (!(ok = mbar_wait(&full[stage], phase, abort_flag, 72))) break;
           tc_fence_after();
@@ -435,77 +455,74 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
           const uint32_t b = a + kLoraShrinkRows * 128;
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_f16_ss(tmem_base, smem_desc_sw128(a + k * 32, 16, 1024),
-                        smem_desc_sw128(b + k * 32, 16, 1024), idesc, kb != kb0 || k != 0 ? 1u : 0u);
+            umma_f16_ss(d, smem_desc_sw128(a + k * 32, 16, 1024), smem_desc_sw128(b + k * 32, 16, 1024),
+                        idesc, kb != kb0 || k != 0 ? 1u : 0u);
           umma_commit(&empty[stage]);
           if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok) umma_commit(tfull);
+        if (ok) umma_commit(&tfull[p & 1]);
       }
     }
-    __syncwarp();
-    const bool done = mbar_wait(tfull, pass & 1, abort_flag, 73);
-    for (int r0 = 0; r0 < R; r0 += 64) {
-      if (warp >= 4 && __all_sync(0xffffffffu, done)) {
-        // Warp q holds tokens [32 q, +32), a lane each; their sums go to CTA q.
-        const int q = warp & 3;
-        tc_fence_after();
-        const int id = s_id[q * 32 + lane];
-        const uint32_t at = map_shared(smem_addr(recv + (rank * 32 + lane) * rs), q);
-        for (int e = 0; e < na; ++e) {
-          const bool is_mine = s_slot[p0 + e] == id;
-          if (!__any_sync(0xffffffffu, is_mine)) continue;
-          for (int c = 0; c < rs; c += 16) {
-            uint32_t v[16];
-            tmem_ld_32x32b_x16(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + e * R + r0 + c, v);
-            tmem_ld_wait();
-            if (is_mine) {
+  } else if (warp >= 4) {
+    // Warp q holds tokens [32 q, +32), a lane each; their sums go to CTA q.
+    const int q = warp & 3;
+    const int id = s_id[q * 32 + lane];
+    const uint32_t at = map_shared(smem_addr(recv + (rank * 32 + lane) * R), q);
+    if (kb1 == kb0 && id >= 0)  // without k-steps this CTA's part of the sum is 0
+      for (int c = 0; c < R; c += 4) st_cluster_u32x4(at + c * 4, 0u, 0u, 0u, 0u);
+    for (int p = 0; p < passes; ++p) {
+      const int p0 = p * per_pass, na = min(per_pass, adapters - p0);
+      const bool done = mbar_wait(&tfull[p & 1], p >> 1 & 1, abort_flag, 73);
+      if (!__all_sync(0xffffffffu, done)) break;
+      tc_fence_after();
+      const uint32_t d = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (p & 1) * kLoraShrinkCols;
+      for (int e = 0; e < na; ++e) {
+        const bool is_mine = s_slot[p0 + e] == id;
+        if (!__any_sync(0xffffffffu, is_mine)) continue;
+        for (int c = 0; c < R; c += 16) {
+          uint32_t v[16];
+          tmem_ld_32x32b_x16(d + e * R + c, v);
+          tmem_ld_wait();
+          if (is_mine) {
 #pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                // A CTA without k-steps has accumulated nothing.
-                const bool some = kb1 > kb0;
-                st_cluster_u32x4(at + (c + j) * 4, some ? v[j] : 0u, some ? v[j + 1] : 0u,
-                                 some ? v[j + 2] : 0u, some ? v[j + 3] : 0u);
-              }
-            }
+            for (int j = 0; j < 16; j += 4)
+              st_cluster_u32x4(at + (c + j) * 4, v[j], v[j + 1], v[j + 2], v[j + 3]);
           }
         }
-        tc_fence_before();
       }
-      cluster_sync();
-      for (int i = tid; i < 32 * rs / 2; i += kLoraThreads) {
-        const int tok = i / (rs / 2), c = i % (rs / 2) * 2;
-        const int id = s_id[rank * 32 + tok];
-        if (id < 0) continue;
-        const int j = s_flag[id];
-        if (j < s_place[p0] || j > s_place[p0 + na - 1]) continue;  // another pass's adapter
-        float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int s = 0; s < kLoraShrinkSplit; ++s) {
-          const float2 v = *reinterpret_cast<const float2*>(recv + (s * 32 + tok) * rs + c);
-          sum.x += v.x;
-          sum.y += v.y;
-        }
-        // Past the adapter's own rank H is 0 whatever x holds.
-        const int own_rank = args.ranks[id];
-        const float scale = args.scales[id];
-        sum.x = r0 + c < own_rank ? sum.x * scale : 0.f;
-        sum.y = r0 + c + 1 < own_rank ? sum.y * scale : 0.f;
-        const int col = j * R + r0 + c;
-        *reinterpret_cast<uint32_t*>(h + col / 64 * group + (t0 - m0 + rank * 32 + tok) * 64 + col % 64) =
-            Pack2<T>::pack(sum.x, sum.y);
-      }
-      cluster_sync();  // read before the next columns overwrite them, or the CTA leaves
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[p & 1]);
     }
+  }
+  __syncwarp();
+  cluster_sync();  // all quarters of this CTA's tokens are here
+  for (int i = tid; i < 32 * R / 2; i += kLoraThreads) {
+    const int tok = i / (R / 2), c = i % (R / 2) * 2, row = rank * 32 + tok;
+    const int id = s_id[row];
+    if (id < 0) continue;
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < kLoraShrinkSplit; ++s) {
+      const float2 v = *reinterpret_cast<const float2*>(recv + (s * 32 + tok) * R + c);
+      sum.x += v.x;
+      sum.y += v.y;
+    }
+    // Past the adapter's own rank H is 0 whatever x holds.
+    sum.x = c < s_own[row] ? sum.x * s_scale[row] : 0.f;
+    sum.y = c + 1 < s_own[row] ? sum.y * s_scale[row] : 0.f;
+    const int col = s_flag[id] * R + c;
+    *reinterpret_cast<uint32_t*>(h + col / 64 * group + (t0 - m0 + row) * 64 + col % 64) =
+        Pack2<T>::pack(sum.x, sum.y);
   }
   // Zeros where a token meets another adapter of its row tile.
   const int vecs = R / 8;
   for (int i = tid; i < 32 * total * vecs; i += kLoraThreads) {
     const int v = i % vecs, e = i / vecs % total, tok = rank * 32 + i / (vecs * total);
-    if (t0 + tok >= args.M || (s_id[tok] >= 0 && s_flag[s_id[tok]] == e)) continue;
+    if (tok >= per || t0 + tok >= args.M || (s_id[tok] >= 0 && s_flag[s_id[tok]] == e)) continue;
     const int col = e * R + v * 8;
     *reinterpret_cast<uint4*>(h + col / 64 * group + (t0 - m0 + tok) * 64 + col % 64) = make_uint4(0, 0, 0, 0);
   }
@@ -518,7 +535,7 @@ __global__ void __launch_bounds__(kLoraThreads, 1)
   __syncthreads();
   if (warp == 3) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, kLoraShrinkCols);
+    tmem_dealloc(tmem_base, 2 * kLoraShrinkCols);
   }
 }
 

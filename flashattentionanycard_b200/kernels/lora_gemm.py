@@ -8,9 +8,9 @@ one adapter per row beside it (the reference has none):
 An ``AdapterBank`` keeps the adapters of a projection in slots on the device, as
 a serving program loads them; ``launch`` runs a batch in which every row names
 its slot, in two kernels: the rows' low-rank vectors, then the projection, whose
-K loop goes on over the adapters that the row tile uses.  Up to 256 rows the
-second kernel streams ``w`` against the tokens (decode); above, it is the
-CTA-pair GEMM (prefill).
+K loop goes on over the adapters that the row tile uses.  With few rows (or few
+tiles) the second kernel streams ``w`` against the tokens (decode); else it is
+the CTA-pair GEMM (prefill).
 """
 
 import math
