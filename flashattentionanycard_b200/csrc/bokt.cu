@@ -1927,6 +1927,8 @@ namespace {
 
 // Rows up to which W is always streamed, beside the shrink of few rows.
 constexpr int kLoraFewRows = 256;
+// Rows up to which W is streamed while the tiles are one wave.
+constexpr int kLoraStreamRows = 1024;
 // Shared memory left to a shrink CTA (rank 16: 9 KB of partials, 7 KB of lists).
 constexpr int kLoraShrinkSmem = 20 * 1024;
 
@@ -1978,13 +1980,15 @@ int lora_plan(int M, int N, int K, int slots, int rank, const DeviceInfo& dev, L
   if (K % 8 != 0 || N % 8 != 0)
     return fail(BOKT_ERR_UNSUPPORTED, "K and N must be multiples of 8 (got %d, %d)", K, N);
   *p = {};
-  // Few rows stream W; so do more of them while the 128 x 128 tiles leave SMs to
-  // split K over (1024 x 1024 of K = 4096: 21 us, 26 on pair tiles; 4096 wide: 35
-  // on pair tiles, 82 streamed).  The shrink of many rows is faster from 257 on
-  // with a few adapters a row tile (512 rows of 9: 27 and 34 us), and slower up to
-  // 700 rows with many (512 rows of 16 adapters of rank 64: 59 and 41).
+  // Few rows stream W; so do up to 1024 while their 128 x 128 tiles are one wave
+  // (K = 4096, streamed and on pair tiles: 512 x 4096 22 and 26 us, 768 x 2048 20.5
+  // and 26, 1024 x 1024 21 and 26; 1024 x 2048 equal; 1000 -> 2056 at 1024 rows
+  // 20.7 and 19.0).  Two waves lose (768 x 4096: 39 and 27), as do 2048 rows of
+  // 1024 columns (28 and 26).  The shrink of many rows is faster from 257 on with
+  // a few adapters a row tile (512 rows of 9 of rank 32: 27 and 34 us), and slower
+  // up to 700 rows with many (512 rows of 16 of rank 64: 59 and 41).
   const long long small_tiles = (long long)((M + 127) / 128) * ((N + 127) / 128);
-  p->stream = M <= kLoraFewRows || small_tiles * 2 <= dev.sm_count;
+  p->stream = M <= kLoraFewRows || (M <= kLoraStreamRows && small_tiles <= dev.sm_count);
   p->shrink_tc = M > kLoraFewRows;
   if (p->stream) {
     const int chunks = (M + 127) / 128;

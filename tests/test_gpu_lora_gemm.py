@@ -250,3 +250,74 @@ def test_streams_graphs_and_two_calls_at_once(cuda_device):
                 g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for (_, o), w in zip(graphs, want))
+
+
+# Either side of the choices of the product (streamed W or pair tiles) and of the shrink.
+EDGES = [
+    (257, 136, 4608, 40, 16, 9), (384, 264, 6400, 12, 32, 7), (1024, 520, 2304, 9, 16, 30),
+    (1024, 136, 2440, 300, 64, None), (1025, 264, 128, 17, 24, None), (1152, 64, 8, 1024, 128, None),
+    (9345, 72, 8, 3, 16, 5),
+]
+
+
+@pytest.mark.parametrize("shape", EDGES)
+def test_projection_at_the_edges_of_its_variants(shape, cuda_device):
+    t, k, n, slots, rank, runs = shape
+    c = Case(t, k, n, slots, rank, runs=runs)
+    out = c.run()
+    c.check(out)
+    assert torch.equal(out, c.run())
+
+
+def test_pair_tiles_report_bad_ids_and_keep_other_rows(cuda_device):
+    c = Case(1300, 136, 520, 20, 24)
+    need = lora_gemm.workspace_bytes(1300, c.bank)
+    c.bank.unload(2)
+    c.ids[3], c.ids[300], c.ids[1299] = 20, -2, 2
+    ids = c.ids.cpu().numpy().copy()
+    ids[(ids == 2) | (ids == 20) | (ids == -2)] = -1
+    clean = c.run()
+    torch.cuda.synchronize()
+    code, detail = _native.device_status(reset=True)
+    assert code == 6 and ids[detail] == -1
+    c.check(clean, ids=ids)
+    c.ids[30] = 1
+    clean = c.run()
+    c.x[5, 3] = float("nan")
+    c.x[30, 9] = float("inf")
+    keep = torch.ones(1300, dtype=torch.bool)
+    keep[5] = keep[30] = False
+    for fill in (0, 255, 127):
+        ws = torch.full((need + 4096,), fill, dtype=torch.uint8, device=cuda_device)
+        out = torch.zeros(1332, 520, dtype=torch.bfloat16, device=cuda_device)
+        lora_gemm.launch(c.x, c.w, c.bank, c.ids, out[16:1316], workspace=ws[:need])
+        assert torch.equal(out[16:1316][keep], clean[keep])
+        assert torch.isnan(out[21]).all() and not torch.isfinite(out[46]).any()
+        assert not out[:16].any() and not out[1316:].any() and (ws[need:] == fill).all()
+    torch.cuda.synchronize()
+    assert _native.device_status(reset=True)[0] == 6
+
+
+def test_pair_tiles_on_streams_and_in_graphs(cuda_device):
+    g = torch.Generator().manual_seed(1)
+    c, d = Case(1100, 512, 512, 5, 16), Case(1100, 512, 512, 5, 16, seed=7)
+    mid, out = torch.empty_like(c.x), torch.empty_like(c.x)
+    c.run(), d.run()
+    lora_gemm.launch(c.x, c.w, c.bank, c.ids, mid)
+    torch.cuda.synchronize()
+    lora_gemm.launch(mid, d.w, d.bank, d.ids, out)
+    want = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lora_gemm.launch(c.x, c.w, c.bank, c.ids, mid)
+        lora_gemm.launch(mid, d.w, d.bank, d.ids, out)
+    other = torch.cuda.Stream()
+    alone = d.run()
+    for _ in range(10):
+        mid.copy_(torch.randn(mid.shape, generator=g))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            beside = d.run()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(beside, alone)
