@@ -372,7 +372,9 @@ __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const 
           dot = fma2(gv[j], v[j], dot);
         }
         // Both sums at once; with n = x r: mean(g w n) = r dot / D.
-        const float r1 = rsqrtf(fmaf(qk_row_sum<L>(ss.x + ss.y), inv_dim, args.eps));
+        // Rows past the unit's heads are zeros: r = 0, or eps = 0 would make them NaN.
+        const float r0 = rsqrtf(fmaf(qk_row_sum<L>(ss.x + ss.y), inv_dim, args.eps));
+        const float r1 = h < at.hend ? r0 : 0.f;
         const float2 rs = both(r1), mean = both(-r1 * inv_dim * qk_row_sum<L>(dot.x + dot.y));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {

@@ -285,3 +285,16 @@ def test_offsets_past_32_bits(cuda_device):
     k.copy_(a["k"])
     qk_norm_rope.launch(q, k, a["q_weight"], a["k_weight"], a["positions"], a["cos_sin"], q, k)
     assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+@pytest.mark.parametrize("shape", [(7, 3, 1, 64, 64), (130, 5, 2, 80, 32), (2500, 7, 3, 96, 48), (9, 3, 2, 37, 36)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_no_epsilon(shape, interleaved, cuda_device):
+    """Heads that do not fill a unit: its idle rows must add nothing where
+    rsqrt(0 + epsilon) is infinite."""
+    a, g = make(*shape, "bf16", seed=3)
+    q_out, k_out = forward(a, interleaved, eps=0.0)
+    check_forward(a, q_out, k_out, "bf16", eps=0.0, interleaved=interleaved)
+    grads = [torch.randn(a[n].shape, generator=g).bfloat16().cuda() for n in ("q", "k")]
+    got = backward(a, *grads, interleaved=interleaved, eps=0.0)
+    check_backward(a, grads, got, "bf16", eps=0.0, interleaved=interleaved)
