@@ -1574,8 +1574,9 @@ int qk_norm_rope_impl(bokt::QkArgs* a, const int64_t* strides, int interleaved, 
     return fail(BOKT_ERR_INVALID, "rot must be even and in [2, head size] (got %d)", a->rot);
   if (!(a->eps >= 0.f) || !(a->eps < 3.0e38f))
     return fail(BOKT_ERR_INVALID, "eps must be finite >= 0");
-  if ((long long)a->tokens * ((long long)a->side[0].heads + a->side[1].heads) > 0x7fffffffLL)
-    return fail(BOKT_ERR_UNSUPPORTED, "more than 2^31 - 1 head rows");
+  // Persistent warps step past the last row by up to a grid: leave the counter room.
+  if ((long long)a->tokens * ((long long)a->side[0].heads + a->side[1].heads) > 0x7fff0000LL)
+    return fail(BOKT_ERR_UNSUPPORTED, "more than 2^31 - 2^16 head rows");
   *blocks = 0;
   int rc = device_info(dev);
   if (rc) return rc;
@@ -1929,6 +1930,8 @@ namespace {
 constexpr int kLoraFewRows = 256;
 // Rows up to which W is streamed while the tiles are one wave.
 constexpr int kLoraStreamRows = 1024;
+// Sizes whose tile arithmetic stays in 32 bits.
+constexpr int kLoraMaxSize = 1 << 30;
 // Shared memory left to a shrink CTA (rank 16: 9 KB of partials, 7 KB of lists).
 constexpr int kLoraShrinkSmem = 20 * 1024;
 
@@ -1979,6 +1982,8 @@ int lora_plan(int M, int N, int K, int slots, int rank, const DeviceInfo& dev, L
     return fail(BOKT_ERR_UNSUPPORTED, "at most %d slots (got %d)", bokt::kLoraMaxSlots, slots);
   if (K % 8 != 0 || N % 8 != 0)
     return fail(BOKT_ERR_UNSUPPORTED, "K and N must be multiples of 8 (got %d, %d)", K, N);
+  if (M > kLoraMaxSize || N > kLoraMaxSize || K > kLoraMaxSize)
+    return fail(BOKT_ERR_UNSUPPORTED, "M, N and K must be at most 2^30 (got %d, %d, %d)", M, N, K);
   *p = {};
   // Few rows stream W; so do up to 1024 while their 128 x 128 tiles are one wave
   // (K = 4096, streamed and on pair tiles: 512 x 4096 22 and 26 us, 768 x 2048 20.5

@@ -17,7 +17,7 @@ import math
 
 from flashattentionanycard_b200 import _native
 
-MAX_SLOTS, RANKS = 1024, (16, 32, 64, 128)
+MAX_SLOTS, MAX_SIZE, RANKS = 1024, 1 << 30, (16, 32, 64, 128)
 
 
 class AdapterBank:
@@ -34,6 +34,8 @@ class AdapterBank:
             raise ValueError(f"slots must be in [1, {MAX_SLOTS}], got {slots}")
         if self.k < 8 or self.n < 8 or self.k % 8 or self.n % 8:
             raise ValueError(f"K and N must be positive multiples of 8 (got {k} and {n})")
+        if self.k > MAX_SIZE or self.n > MAX_SIZE:
+            raise ValueError(f"K and N must be at most {MAX_SIZE} (got {k} and {n})")
         if not 1 <= int(max_rank) <= RANKS[-1]:
             raise ValueError(f"max_rank must be in [1, {RANKS[-1]}], got {max_rank}")
         _native.dtype_code(dtype)
@@ -109,6 +111,8 @@ def launch(x, w, bank, ids, out, workspace=None):
     n = w.shape[1]
     if w.shape[0] != k or out.shape != (m, n):
         raise ValueError(f"shape mismatch: x {tuple(x.shape)}, w {tuple(w.shape)}, out {tuple(out.shape)}")
+    if m > MAX_SIZE:
+        raise ValueError(f"at most {MAX_SIZE} rows (got {m})")
     if k != bank.k or n != bank.n:
         raise ValueError(f"the bank's adapters are for a [{bank.k}, {bank.n}] projection, not [{k}, {n}]")
     if ids.dtype != torch.int32 or ids.shape != (m,) or not ids.is_contiguous():

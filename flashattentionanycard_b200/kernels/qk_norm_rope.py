@@ -23,14 +23,16 @@ import struct
 
 from flashattentionanycard_b200 import _native
 
+MAX_HEAD_ROWS = (1 << 31) - (1 << 16)
+
 
 def rope_table(rows, rot, base=10000.0, device="cuda"):
     """fp32 [rows, rot]: cosines and sines of p * base^(-2 i / rot), angles in 64 bits."""
     import torch
 
     rows, rot = int(rows), int(rot)
-    if rows < 0 or rot < 2 or rot % 2:
-        raise ValueError("rows must be non-negative and rot even and positive")
+    if not 0 <= rows < 1 << 31 or not 2 <= rot < 1 << 31 or rot % 2:
+        raise ValueError("rows must be non-negative, rot even and positive, both below 2^31")
     if not (math.isfinite(base) and base > 0):
         raise ValueError("base must be finite and positive")
     out = torch.empty((rows, rot), device=device, dtype=torch.float32)
@@ -89,9 +91,11 @@ def _check(q, k, q_weight, k_weight, positions, cos_sin, epsilon):
     qs, ks = q.shape, k.shape
     if len(qs) != 3 or len(ks) != 3:
         raise ValueError(f"q and k must be [tokens, heads, head size], got {tuple(qs)} and {tuple(ks)}")
-    t, _, d = qs
+    t, h, d = qs
     if ks[0] != t or ks[2] != d:
         raise ValueError(f"shape mismatch: q {tuple(qs)}, k {tuple(ks)}")
+    if t * (h + ks[1]) > MAX_HEAD_ROWS or t > MAX_HEAD_ROWS:
+        raise ValueError(f"at most {MAX_HEAD_ROWS} head rows (got {t} tokens of {h} + {ks[1]} heads)")
     index = q.get_device()
     _weight("q_weight", q_weight, d, q.dtype, index)
     _weight("k_weight", k_weight, d, q.dtype, index)
@@ -102,6 +106,8 @@ def _check(q, k, q_weight, k_weight, positions, cos_sin, epsilon):
     if cos_sin.dtype != torch.float32 or len(table) != 2 or not cos_sin.is_contiguous():
         raise ValueError("cos_sin must be a contiguous fp32 [positions, rot] tensor")
     rot = table[1]
+    if table[0] > MAX_HEAD_ROWS:
+        raise ValueError(f"cos_sin must have at most {MAX_HEAD_ROWS} rows, got {table[0]}")
     if rot < 2 or rot % 2 or rot > d:
         raise ValueError(f"rot (cos_sin's width) must be even and in [2, {d}], got {rot}")
     if not (epsilon >= 0 and math.isfinite(epsilon)):

@@ -218,7 +218,8 @@ int bokt_rmsnorm_gemm(const void* X, const void* B_folded, void* C, float* row_s
  * operand), the sum once.  out must not overlap x.  lora_b must be finite:
  * rows of other adapters multiply it by zero.  An id outside [-1, slots) or of an empty slot sets the
  * device status word (code 6) and its row gets x W alone.  rank: 16, 32, 64 or
- * 128; slots <= 1024; K and N multiples of 8; 16-byte aligned pointers.
+ * 128; slots <= 1024; K and N multiples of 8; M, K and N up to 2^30; 16-byte
+ * aligned pointers.
  * workspace: bokt_lora_gemm_workspace_bytes(...) bytes of device scratch,
  * 256-byte aligned, contents free before and after; calls that overlap on the
  * GPU need one each.  The product is that of kernels/gemm.py:7-40; adapters
@@ -243,7 +244,7 @@ int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void*
  * be q / k themselves (same strides).  A position outside the table sets the
  * device status word (code 5) and leaves that token's heads unwritten.
  * strides[8]: q row, q head, q_out row, q_out head, then the same of k.
- * dim in [2, 1024], rot even; dim a multiple of 8 up to 256 with 16-byte
+ * tokens * (heads + kv_heads) up to 2^31 - 2^16; dim in [2, 1024], rot even; dim a multiple of 8 up to 256 with 16-byte
  * aligned rows and rot a multiple of 16 (8 interleaved) runs vectorised.  The
  * RMSNorm of kernels/rmsnorm.py:22-25 applied to each head; the rotation has
  * no counterpart in the reference.

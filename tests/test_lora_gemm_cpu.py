@@ -109,3 +109,16 @@ def test_c_abi_argument_errors_need_no_gpu():
     assert rc(slots=1025) == 2 and rc(k=12) == 2 and rc(n=4) == 2
     assert rc(m=0) == 0
     assert rc() == 1 and b"null" in lib.bokt_last_error()
+
+
+def test_sizes_past_32_bits_are_refused():
+    lib, most = _native.load(), 1 << 30
+    for sizes in ((most + 1, 24, 16), (8, most + 8, 16), (8, 24, most + 8)):
+        assert lib.bokt_lora_gemm_workspace_bytes(*sizes, 4, 16) == -1
+    null = [None] * 8
+    assert lib.bokt_lora_gemm(*null, most + 1, 24, 16, 4, 16, _native.BF16, None, 0, None) != 0
+    assert b"2^30" in lib.bokt_last_error()
+    b = bank()
+    x, w, ids = torch.zeros(1, 16, dtype=BF), torch.zeros(16, 24, dtype=BF), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="rows"):
+        lora_gemm.launch(x.expand(most + 1, 16), w, b, ids, torch.zeros(1, 24, dtype=BF).expand(most + 1, 24))

@@ -87,3 +87,20 @@ def test_one_buffer_for_both_weight_gradients_is_refused():
     both = torch.zeros(16)
     with pytest.raises(ValueError, match="separate"):
         call(backward=True, dq_weight=both, dk_weight=both)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_sizes_past_32_bits_are_refused(backward):
+    bf = torch.bfloat16
+    many = torch.zeros(1, 1, 16, dtype=bf).expand(3, 1 << 30, 16)
+    with pytest.raises(ValueError, match="head rows"):
+        call(backward=backward, q=many)
+    with pytest.raises(ValueError, match="head rows"):
+        call(backward=backward, k=many)
+    none = torch.zeros(1, 0, 16, dtype=bf).expand(1 << 32, 0, 16)
+    with pytest.raises(ValueError, match="head rows"):
+        call(backward=backward, q=none, k=none)
+    with pytest.raises(ValueError, match="2\\^31"):
+        qk_norm_rope.rope_table(1 << 31, 64)
+    with pytest.raises(ValueError, match="2\\^31"):
+        qk_norm_rope.rope_table(4, 1 << 31)
