@@ -244,10 +244,11 @@ int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void*
  * be q / k themselves (same strides).  A position outside the table sets the
  * device status word (code 5) and leaves that token's heads unwritten.
  * strides[8]: q row, q head, q_out row, q_out head, then the same of k.
- * tokens * (heads + kv_heads) up to 2^31 - 2^16; dim in [2, 1024], rot even; dim a multiple of 8 up to 256 with 16-byte
- * aligned rows and rot a multiple of 16 (8 interleaved) runs vectorised.  The
- * RMSNorm of kernels/rmsnorm.py:22-25 applied to each head; the rotation has
- * no counterpart in the reference.
+ * tokens * (heads + kv_heads) up to 2^31 - 2^16; dim in [2, 1024], rot even;
+ * dim a multiple of 8 up to 256 with 16-byte aligned rows and rot a multiple
+ * of 16 (8 interleaved) runs vectorised.  The RMSNorm of
+ * kernels/rmsnorm.py:22-25 applied to each head; the rotation has no
+ * counterpart in the reference.
  */
 int bokt_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight,
                       const void* positions, int positions_i64, const float* cos_sin,

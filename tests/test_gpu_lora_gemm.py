@@ -321,3 +321,22 @@ def test_pair_tiles_on_streams_and_in_graphs(cuda_device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(beside, alone)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """x and out of more than 2^31 elements: 1000 rows over and over.  Odd waves
+    of pair tiles walk K downwards, so a row's sum may be taken in either order:
+    every repeat is held to the bound, which covers any order."""
+    c = Case(1000, 8192, 8192, 12, 16)
+    t = 263_000
+    x, ids = c.x.repeat(t // 1000, 1), c.ids.repeat(t // 1000)
+    assert x.numel() > 2**31
+    out = torch.full_like(x, float("nan"))
+    lora_gemm.launch(x, c.w, c.bank, ids, out)
+    del x
+    some = torch.arange(0, 1000, 37)
+    c.x, c.ids = c.x[some], c.ids[some]
+    ref, tol = (torch.from_numpy(v).cuda() for v in c.bound())
+    for block in out.view(t // 1000, 1000, -1):
+        assert ((block[some].double() - ref).abs() <= tol).all()
+    assert torch.isfinite(out[:1000]).all() and torch.isfinite(out[-1000:]).all()
