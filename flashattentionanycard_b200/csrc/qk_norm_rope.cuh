@@ -20,7 +20,7 @@
 // into 16 registers and serve all of them, and R row loads are in flight per
 // lane.  Measured at (32 + 8) heads x 128 bf16: forward of 16384 tokens 62-63 us,
 // 5.4 TB/s with the table (without overlap of launches: one loop of R = 4 77 us,
-// two 68, four 64; R = 2 70-82); backward of 8192 tokens 57 us, 4.5 TB/s (one
+// two 68, four 64; R = 2 70-82); backward of 8192 tokens 58 us, 4.4 TB/s (one
 // loop 64, two 57, four 58; R = 2 58-83; 24 warps an SM instead of 16: 62).
 #pragma once
 
