@@ -1520,7 +1520,7 @@ cudaError_t launch_qk_any(const bokt::QkArgs& a, int sm_count, int* blocks, cuda
                 size_t(4) * 3 * a.dim * 4, s, a);
 }
 
-template <typename T, int L, bool PAIRS, int R, bool GRAD>
+template <typename T, int L, bool PAIRS, bool PART, int R, bool GRAD>
 cudaError_t launch_qk_vec(bokt::QkArgs a, int sm_count, int* blocks, cudaStream_t s) {
   // As many rows behind one load of the angles as leave every SM two rounds
   // of 32 warps, up to the measured best (four loops forward, two backward).
@@ -1536,13 +1536,13 @@ cudaError_t launch_qk_vec(bokt::QkArgs a, int sm_count, int* blocks, cudaStream_
     if (grid > (long long)kQkGradBlocksPerSm * sm_count)
       grid = (long long)kQkGradBlocksPerSm * sm_count;
     *blocks = int(grid);
-    auto* kernel = bokt::qk_norm_rope_grad_kernel<T, L, PAIRS, R>;
+    auto* kernel = bokt::qk_norm_rope_grad_kernel<T, L, PAIRS, PART, R>;
     const int smem = bokt::qk_grad_smem_bytes<L, R>();
     if (ensure_smem(reinterpret_cast<const void*>(kernel), smem)) return cudaErrorInvalidValue;
     return launch(kernel, dim3(unsigned(grid)), dim3(bokt::kQkThreads), smem, s, a);
   } else {
     *blocks = 0;
-    return launch(bokt::qk_norm_rope_kernel<T, L, PAIRS, R>,
+    return launch(bokt::qk_norm_rope_kernel<T, L, PAIRS, PART, R>,
                   dim3(unsigned((u0 + u1 + bokt::kQkWarps - 1) / bokt::kQkWarps)),
                   dim3(bokt::kQkThreads), 0, s, a);
   }
@@ -1554,13 +1554,16 @@ cudaError_t launch_qk(const bokt::QkArgs& a, bool vec, int sm_count, int* blocks
   // Few head rows: one row per lane group, so that the call spreads over the
   // SMs; many: four loads in flight per lane.
   const bool few = (long long)a.tokens * (a.side[0].heads + a.side[1].heads) < 64ll * sm_count;
-#define BOKT_QK(L) \
-  (few ? launch_qk_vec<T, L, PAIRS, 1, GRAD>(a, sm_count, blocks, s) \
-       : launch_qk_vec<T, L, PAIRS, 4, GRAD>(a, sm_count, blocks, s))
+#define BOKT_QK_PART(L, PART) \
+  (few ? launch_qk_vec<T, L, PAIRS, PART, 1, GRAD>(a, sm_count, blocks, s) \
+       : launch_qk_vec<T, L, PAIRS, PART, 4, GRAD>(a, sm_count, blocks, s))
+  // PART, but for neighbours that all turn (see the kernel).
+#define BOKT_QK(L) (!PAIRS || a.rot < a.dim ? BOKT_QK_PART(L, true) : BOKT_QK_PART(L, !PAIRS))
   if (a.dim <= 64) return BOKT_QK(8);
   if (a.dim <= 128) return BOKT_QK(16);
   return BOKT_QK(32);
 #undef BOKT_QK
+#undef BOKT_QK_PART
 }
 
 int qk_norm_rope_impl(bokt::QkArgs* a, const int64_t* strides, int interleaved, int dtype,

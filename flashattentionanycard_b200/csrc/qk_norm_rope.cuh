@@ -145,26 +145,30 @@ __device__ __forceinline__ void qk_load_angles(const float* row, int rot, int i,
 }
 
 // The 8 elements that turn with this lane's: the partner lane's row bits (four
-// shuffles of packed pairs), or the neighbours of the lane's own pairs.  Lanes
-// past rot are their own partner, with c = 1 and s = 0.
+// shuffles of packed pairs), or the neighbours of the lane's own pairs; zeros
+// for a lane that does not turn (its s is 0, but 0 times an infinity is not).
 template <typename T, bool PAIRS>
 __device__ __forceinline__ void qk_partner(const uint4& raw, const float2 (&v)[4], int partner,
-                                           float2 (&o)[4]) {
+                                           bool turns, float2 (&o)[4]) {
   if constexpr (PAIRS) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = make_float2(v[j].y, v[j].x);
+    for (int j = 0; j < 4; ++j) o[j] = turns ? make_float2(v[j].y, v[j].x) : both(0.f);
   } else {
     uint4 p;
     p.x = __shfl_sync(0xffffffffu, raw.x, partner);
     p.y = __shfl_sync(0xffffffffu, raw.y, partner);
     p.z = __shfl_sync(0xffffffffu, raw.z, partner);
     p.w = __shfl_sync(0xffffffffu, raw.w, partner);
-    qk_unpack<T>(p, o);
+    qk_unpack<T>(turns ? p : make_uint4(0, 0, 0, 0), o);
   }
 }
 
 // Head units: unit u covers heads [chunk * HPU, +HPU) of token u / chunks.
-template <typename T, int L, bool PAIRS, int R>
+// PART: rot is less than the head size.  A rotation of whole heads leaves the
+// zeros of qk_partner out, which for neighbours are eight selects a row
+// ((32 + 8) heads x 128, forward of 16384 tokens 57.9 us without and 60.9 with
+// them, backward of 8192 54.8 and 56.2; halves within 0.3 either way: always PART).
+template <typename T, int L, bool PAIRS, bool PART, int R>
 __global__ void __launch_bounds__(kQkThreads, 4) qk_norm_rope_kernel(const QkArgs args) {
   constexpr int S = 32 / L;
   pdl_allow_next();
@@ -210,7 +214,7 @@ __global__ void __launch_bounds__(kQkThreads, 4) qk_norm_rope_kernel(const QkArg
   {
     float2 w[4], pw[4];
     qk_unpack<T>(wraw, w);
-    qk_partner<T, PAIRS>(wraw, w, partner, pw);
+    qk_partner<T, PAIRS>(wraw, w, partner, !PART || turns, pw);
 #pragma unroll
     for (int j = 0; j < 4; ++j) ang.c[j] = mul2(ang.c[j], w[j]), ang.s[j] = mul2(ang.s[j], pw[j]);
   }
@@ -221,7 +225,9 @@ __global__ void __launch_bounds__(kQkThreads, 4) qk_norm_rope_kernel(const QkArg
       const int h = h0 + r * S;
       float2 v[4], o[4], ss = both(0.f);
       qk_unpack<T>(raw[r], v);
-      qk_partner<T, PAIRS>(raw[r], v, partner, o);
+      // Past rot a lane of halves is its own partner: an infinity there is NaN as
+      // it is (its row's rsqrt is 0), so only neighbours need the zeros.
+      qk_partner<T, PAIRS>(raw[r], v, partner, !PAIRS || !PART || turns, o);
 #pragma unroll
       for (int j = 0; j < 4; ++j) ss = fma2(v[j], v[j], ss);
       const float2 rs = both(rsqrtf(fmaf(qk_row_sum<L>(ss.x + ss.y), inv_dim, args.eps)));
@@ -281,7 +287,7 @@ __host__ __device__ constexpr int qk_grad_smem_bytes() {
 // and lane until the end, are summed over the block's rows in shared memory and
 // leave as one partial row per block and side, which
 // qk_norm_rope_dweight_kernel adds in block order.
-template <typename T, int L, bool PAIRS, int R>
+template <typename T, int L, bool PAIRS, bool PART, int R>
 __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const QkArgs args) {
   constexpr int S = 32 / L;
   extern __shared__ uint4 qk_ring[];
@@ -362,7 +368,7 @@ __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_grad_kernel(const 
         qk_unpack<T>(xr, v);
         qk_unpack<T>(gr, gv);
         qk_unpack<T>(wraw, w);
-        qk_partner<T, PAIRS>(gr, gv, partner, o);
+        qk_partner<T, PAIRS>(gr, gv, partner, !PART || turns, o);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           gv[j] = fma2(gv[j], ang.c[j], mul2(o[j], ang.s[j]));  // turned back

@@ -298,3 +298,39 @@ def test_no_epsilon(shape, interleaved, cuda_device):
     grads = [torch.randn(a[n].shape, generator=g).bfloat16().cuda() for n in ("q", "k")]
     got = backward(a, *grads, interleaved=interleaved, eps=0.0)
     check_backward(a, grads, got, "bf16", eps=0.0, interleaved=interleaved)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("t, d, rot", [(6, 64, 32), (6, 80, 16), (700, 256, 64), (5, 37, 12)])
+def test_infinities_past_the_rotation_stay_in_their_column(t, d, rot, interleaved, cuda_device):
+    """Past rot nothing mixes: an infinity there reaches no other column, in
+    either form of the pairs, from the values, the weights or the gradient."""
+    h, col = 20 if t > 100 else 3, rot + 3
+    a, g = make(t, h, 1, d, rot, "bf16")
+    a["q"], a["k"] = a["q"].contiguous(), a["k"].contiguous()
+    grads = [torch.randn(*a[n].shape, generator=g).bfloat16().to(cuda_device) for n in ("q", "k")]
+    others = [c for c in range(d) if c != col]
+    clean, clean_grad = forward(a, interleaved), backward(a, *grads, interleaved)
+
+    bad = {**a, "q": a["q"].clone()}
+    bad["q"][2, 1, col] = float("inf")  # x / inf is 0, inf / inf is NaN
+    out = forward(bad, interleaved)[0]
+    assert torch.equal(out[2, 1, others], torch.zeros_like(out[2, 1, others])) and torch.isnan(out[2, 1, col])
+    # Backward the row's statistics are gone; it adds to no other column of the weights' gradient.
+    silent = [grads[0].clone(), grads[1]]
+    silent[0][2, 1] = 0
+    without, got = backward(a, *silent, interleaved)[2], backward(bad, *grads, interleaved)
+    assert torch.equal(got[2][others], without[others]) and torch.isnan(got[2][col])
+
+    bad = {**a, "q_weight": a["q_weight"].clone()}
+    bad["q_weight"][col] = float("inf")
+    out = forward(bad, interleaved)[0]
+    assert torch.equal(out[..., others], clean[0][..., others]) and torch.isinf(out[..., col]).all()
+
+    grads[0][2, 1, col] = float("inf")
+    got = backward(a, *grads, interleaved)
+    assert torch.equal(got[2][others], clean_grad[2][others]) and torch.isinf(got[2][col])
+    assert torch.equal(got[1], clean_grad[1]) and torch.equal(got[3], clean_grad[3])
+    rows = torch.ones(t, h, dtype=torch.bool)
+    rows[2, 1] = False
+    assert torch.equal(got[0][rows], clean_grad[0][rows])
