@@ -25,7 +25,9 @@ ERRORS = {
     3: "invalid launch configuration",
     4: "CUDA error",
     5: "device-reported failure",
+    6: "overlapping memory",
 }
+ERR_OVERLAP = 6
 
 # Public parameter names (search-space keys) -> bokt_params fields.
 PARAM_FIELDS = {
@@ -174,10 +176,12 @@ def load():
 
 
 def check(rc, what):
-    """Turn a non-zero status into RuntimeError carrying bokt_last_error()."""
+    """Turn a non-zero status into RuntimeError (ValueError for operands that
+    overlap) carrying bokt_last_error()."""
     if rc != 0:
         message = load().bokt_last_error().decode(errors="replace")
-        raise RuntimeError(f"{what} failed ({ERRORS.get(rc, rc)}): {message}")
+        error = ValueError if rc == ERR_OVERLAP else RuntimeError
+        raise error(f"{what} failed ({ERRORS.get(rc, rc)}): {message}")
 
 
 def make_params(params):

@@ -5,10 +5,12 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <numeric>
 
 #include "../../include/bokt.h"
 #include "bokt_device.cuh"
@@ -1566,8 +1568,82 @@ cudaError_t launch_qk(const bokt::QkArgs& a, bool vec, int sm_count, int* blocks
 #undef BOKT_QK_PART
 }
 
+// Memory of one operand of T x H head rows, in bytes.
+struct QkSpan {
+  const char* p;
+  int64_t row, head, width;
+  int T, H;
+};
+
+QkSpan qk_span(const void* p, int64_t row, int64_t head, const bokt::QkArgs& a, int heads) {
+  QkSpan s = {static_cast<const char*>(p), 2 * row, 2 * head, 2 * (int64_t)a.dim, a.tokens, heads};
+  if (s.T <= 1) s.row = 0;  // a stride that nothing takes
+  if (s.H <= 1) s.head = 0;
+  if (s.row < 0) s.p += (s.T - 1) * s.row, s.row = -s.row;
+  if (s.head < 0) s.p += (s.H - 1) * s.head, s.head = -s.head;
+  return s;
+}
+
+bool qk_same(const QkSpan& a, const QkSpan& b) { return a.p == b.p && a.row == b.row && a.head == b.head; }
+
+// Whether the two share no byte: separate ranges, or blocks that never meet
+// modulo a stride they have in common (heads beside each other in every token's
+// row, token rows beside each other in every head, or all strides' divisor).
+// False also where none of these shows it.
+bool qk_apart(const QkSpan& a, const QkSpan& b) {
+  if (!a.T || !a.H || !b.T || !b.H) return true;
+  using wide = __int128;
+  const wide gap = (wide) reinterpret_cast<intptr_t>(b.p) - reinterpret_cast<intptr_t>(a.p);
+  auto row_block = [](const QkSpan& s) { return (wide)(s.H - 1) * s.head + s.width; };
+  auto head_block = [](const QkSpan& s) { return (wide)(s.T - 1) * s.row + s.width; };
+  auto end = [&](const QkSpan& s) { return (wide)(s.T - 1) * s.row + row_block(s); };
+  if (gap >= end(a) || -gap >= end(b)) return true;
+  auto beside = [&](wide period, wide ea, wide eb) {
+    if (period <= 0) return false;
+    const wide at = (gap % period + period) % period;
+    return at >= ea && at + eb <= period;
+  };
+  // A span of one token (or head) may be taken to step like the other.
+  if (a.row == b.row || a.T == 1 || b.T == 1)
+    if (beside(std::max(a.row, b.row), row_block(a), row_block(b))) return true;
+  if (a.head == b.head || a.H == 1 || b.H == 1)
+    if (beside(std::max(a.head, b.head), head_block(a), head_block(b))) return true;
+  return beside(std::gcd(std::gcd(a.row, b.row), std::gcd(a.head, b.head)), a.width, b.width);
+}
+
+// Outputs are written while other rows are still read: they share no memory
+// with each other or with an input, but for each side's own inputs, whole (a
+// row is read and written by one warp).  dw: the weights' gradients, or null.
+int qk_check_overlap(const bokt::QkArgs& a, bool grad, const float* const* dw) {
+  const char* const outs[2] = {grad ? "dq" : "q_out", grad ? "dk" : "k_out"};
+  const char* const ins[4] = {"q", "k", "dq_out", "dk_out"};
+  QkSpan out[2], in[4];
+  for (int i = 0; i < 2; ++i) {
+    const bokt::QkSide& s = a.side[i];
+    out[i] = qk_span(s.out, s.out_row, s.out_head, a, s.heads);
+    in[i] = qk_span(s.x, s.x_row, s.x_head, a, s.heads);
+    in[2 + i] = qk_span(s.g, s.g_row, s.g_head, a, grad ? s.heads : 0);
+  }
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 4; ++j)
+      if (!((j & 1) == i && qk_same(out[i], in[j])) && !qk_apart(out[i], in[j]))
+        return fail(BOKT_ERR_OVERLAP, "%s must not overlap %s%s", outs[i], ins[j],
+                    (j & 1) == i ? " (unless it is the same view)" : "");
+  if (!qk_apart(out[0], out[1])) return fail(BOKT_ERR_OVERLAP, "%s must not overlap %s", outs[0], outs[1]);
+  if (!dw) return BOKT_OK;
+  const char* const dws[2] = {"dq_weight", "dk_weight"};
+  QkSpan w[2];
+  for (int i = 0; i < 2; ++i) w[i] = {reinterpret_cast<const char*>(dw[i]), 0, 0, 4 * (int64_t)a.dim, 1, 1};
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2; ++j)
+      if (!qk_apart(w[i], out[j])) return fail(BOKT_ERR_OVERLAP, "%s must not overlap %s", dws[i], outs[j]);
+  if (!qk_apart(w[0], w[1])) return fail(BOKT_ERR_OVERLAP, "dq_weight must not overlap dk_weight");
+  return BOKT_OK;
+}
+
 int qk_norm_rope_impl(bokt::QkArgs* a, const int64_t* strides, int interleaved, int dtype,
-                      bool grad, void* stream, int* blocks, DeviceInfo* dev) {
+                      const float* const* dw, void* stream, int* blocks, DeviceInfo* dev) {
+  const bool grad = dw != nullptr;
   if (dtype != BOKT_FP16 && dtype != BOKT_BF16) return fail(BOKT_ERR_INVALID, "dtype %d", dtype);
   if (a->tokens < 0 || a->side[0].heads < 0 || a->side[1].heads < 0 || a->table_rows < 0)
     return fail(BOKT_ERR_INVALID, "negative size");
@@ -1580,23 +1656,27 @@ int qk_norm_rope_impl(bokt::QkArgs* a, const int64_t* strides, int interleaved, 
   // Persistent warps step past the last row by up to a grid: leave the counter room.
   if ((long long)a->tokens * ((long long)a->side[0].heads + a->side[1].heads) > 0x7fff0000LL)
     return fail(BOKT_ERR_UNSUPPORTED, "more than 2^31 - 2^16 head rows");
-  *blocks = 0;
-  int rc = device_info(dev);
-  if (rc) return rc;
-  if (a->tokens == 0 || a->side[0].heads + a->side[1].heads == 0) return BOKT_OK;
-  if (!strides || !a->positions || !a->cos_sin) return fail(BOKT_ERR_INVALID, "null pointer");
+  const bool empty = a->tokens == 0 || a->side[0].heads + a->side[1].heads == 0;
   bool vec = a->dim % 8 == 0 && a->dim <= bokt::kQkMaxVecDim && a->rot % (interleaved ? 8 : 16) == 0 &&
              aligned16(a->cos_sin);
-  for (int i = 0; i < 2; ++i) {
-    bokt::QkSide& s = a->side[i];
-    if (s.heads && (!s.x || !s.w || !s.out || (grad && !s.g)))
-      return fail(BOKT_ERR_INVALID, "null pointer");
-    const int64_t* st = strides + (grad ? 6 : 4) * i;
-    s.x_row = st[0], s.x_head = st[1];
-    s.out_row = st[2], s.out_head = st[3];
-    if (grad) s.g_row = st[4], s.g_head = st[5];
-    vec = vec && (s.heads == 0 || qk_strides_vec(s));
+  int rc;
+  if (!empty) {
+    if (!strides || !a->positions || !a->cos_sin) return fail(BOKT_ERR_INVALID, "null pointer");
+    for (int i = 0; i < 2; ++i) {
+      bokt::QkSide& s = a->side[i];
+      if (s.heads && (!s.x || !s.w || !s.out || (grad && !s.g)))
+        return fail(BOKT_ERR_INVALID, "null pointer");
+      const int64_t* st = strides + (grad ? 6 : 4) * i;
+      s.x_row = st[0], s.x_head = st[1];
+      s.out_row = st[2], s.out_head = st[3];
+      if (grad) s.g_row = st[4], s.g_head = st[5];
+      vec = vec && (s.heads == 0 || qk_strides_vec(s));
+    }
   }
+  if ((rc = qk_check_overlap(*a, grad, dw))) return rc;
+  *blocks = 0;
+  if ((rc = device_info(dev))) return rc;
+  if (empty) return BOKT_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
 #define BOKT_QK(T, P) \
@@ -1629,7 +1709,7 @@ int bokt_qk_norm_rope(const void* q, const void* k, const void* q_weight, const 
   a.tokens = tokens, a.dim = dim, a.rot = rot, a.eps = eps;
   int blocks;
   DeviceInfo dev;
-  return qk_norm_rope_impl(&a, strides, interleaved, dtype, false, stream, &blocks, &dev);
+  return qk_norm_rope_impl(&a, strides, interleaved, dtype, nullptr, stream, &blocks, &dev);
 }
 
 int64_t bokt_qk_norm_rope_workspace_bytes(int dim) {
@@ -1657,12 +1737,13 @@ int bokt_qk_norm_rope_backward(const void* dq_out, const void* dk_out, const voi
   a.partials = static_cast<float*>(workspace);
   if (!dq_weight || !dk_weight || !workspace) return fail(BOKT_ERR_INVALID, "null pointer");
   DeviceInfo dev;
-  int rc = device_info(&dev);
-  if (rc) return rc;
-  if (workspace_bytes < (int64_t)kQkGradBlocksPerSm * dev.sm_count * 2 * dim * 4)
-    return fail(BOKT_ERR_INVALID, "workspace too small (%lld bytes)", (long long)workspace_bytes);
   int blocks;
-  rc = qk_norm_rope_impl(&a, strides, interleaved, dtype, true, stream, &blocks, &dev);
+  const float* const dw[2] = {dq_weight, dk_weight};
+  int rc = device_info(&dev);
+  if (rc == BOKT_OK && workspace_bytes < (int64_t)kQkGradBlocksPerSm * dev.sm_count * 2 * dim * 4)
+    return fail(BOKT_ERR_INVALID, "workspace too small (%lld bytes)", (long long)workspace_bytes);
+  // Without a device the sizes and the overlaps are still looked at first.
+  rc = qk_norm_rope_impl(&a, strides, interleaved, dtype, dw, stream, &blocks, &dev);
   if (rc) return rc;
   // No rows: the weight gradients are zero.
   cudaError_t e = launch(bokt::qk_norm_rope_dweight_kernel, dim3(unsigned((dim + 31) / 32), 2),

@@ -118,7 +118,8 @@ def _check(q, k, q_weight, k_weight, positions, cos_sin, epsilon):
 
 
 def launch(q, k, q_weight, k_weight, positions, cos_sin, q_out, k_out, epsilon=1e-6, interleaved=False):
-    """q_out, k_out = rotated norms of q's and k's heads (q_out may be q, k_out may be k)."""
+    """q_out, k_out = rotated norms of q's and k's heads (q_out may be q, k_out
+    may be k; outputs that overlap otherwise are a ValueError)."""
     import torch
 
     qs, ks, rot, rows, index, i64 = _check(q, k, q_weight, k_weight, positions, cos_sin, epsilon)
@@ -142,9 +143,10 @@ def launch(q, k, q_weight, k_weight, positions, cos_sin, q_out, k_out, epsilon=1
 
 def launch_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, cos_sin, dq, dk, dq_weight,
                     dk_weight, epsilon=1e-6, interleaved=False):
-    """Gradients of ``launch``: dq, dk (q's dtype; dq may be dq_out, dk may be
-    dk_out) and dq_weight, dk_weight (fp32 [D], overwritten, summed in a fixed
-    order: the same inputs give the same bits)."""
+    """Gradients of ``launch``: dq, dk (q's dtype; dq may be dq_out or q, dk may
+    be dk_out or k; any other overlap is a ValueError) and dq_weight, dk_weight
+    (fp32 [D], overwritten, summed in a fixed order: the same inputs give the
+    same bits)."""
     import torch
 
     qs, ks, rot, rows, index, i64 = _check(q, k, q_weight, k_weight, positions, cos_sin, epsilon)

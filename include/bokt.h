@@ -53,6 +53,7 @@ extern "C" {
 #define BOKT_ERR_CONFIG 3      /* launch parameters outside the kernel's domain */
 #define BOKT_ERR_CUDA 4        /* a CUDA runtime/driver call failed */
 #define BOKT_ERR_DEVICE 5      /* a kernel reported a timeout through the device status word */
+#define BOKT_ERR_OVERLAP 6     /* an output shares memory with another output or an input */
 
 /* kernel identifiers for bokt_kernel_attrs */
 #define BOKT_KERNEL_GEMM 0
@@ -241,7 +242,8 @@ int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void*
  * (i, i + rot / 2), or (2 i, 2 i + 1) with interleaved, turns by the angle
  * whose cosine is cos_sin[p][i] and whose sine is cos_sin[p][rot / 2 + i]
  * (fp32 [table_rows, rot]).  fp32 arithmetic, one rounding.  q_out / k_out may
- * be q / k themselves (same strides).  A position outside the table sets the
+ * be q / k themselves (same strides); any other overlap of an output with
+ * another or with q or k is BOKT_ERR_OVERLAP.  A position outside the table sets the
  * device status word (code 5) and leaves that token's heads unwritten.
  * strides[8]: q row, q head, q_out row, q_out head, then the same of k.
  * tokens * (heads + kv_heads) up to 2^31 - 2^16; dim in [2, 1024], rot even;
@@ -257,8 +259,9 @@ int bokt_qk_norm_rope(const void* q, const void* k, const void* q_weight, const 
                       float eps, int dtype, void* stream);
 
 /*
- * Gradients of bokt_qk_norm_rope: dq, dk (may be dq_out / dk_out themselves)
- * and the weights' gradients dq_weight, dk_weight (fp32 [dim], apart, overwritten;
+ * Gradients of bokt_qk_norm_rope: dq, dk (may be dq_out / dk_out, or q / k,
+ * themselves; any other overlap is BOKT_ERR_OVERLAP) and the weights' gradients
+ * dq_weight, dk_weight (fp32 [dim], apart from each other and from dq and dk, overwritten;
  * summed in a fixed order for a given device and shape).  The row statistics
  * are recomputed from q and k.  strides[12]: q row, q head, dq row, dq head,
  * dq_out row, dq_out head, then the same of k.  A token whose position is

@@ -334,3 +334,57 @@ def test_infinities_past_the_rotation_stay_in_their_column(t, d, rot, interleave
     rows = torch.ones(t, h, dtype=torch.bool)
     rows[2, 1] = False
     assert torch.equal(got[0][rows], clean_grad[0][rows])
+
+
+def test_outputs_over_other_operands_are_refused(cuda_device):
+    """Any memory in common but a side's own view, whole, is an error, and nothing runs."""
+    t, h, hk, d = 30, 4, 2, 64
+    a, g = make(t, h, hk, d, d, "bf16")
+    want = forward(a)
+    buf = torch.zeros(4 * t, h + hk, d, dtype=torch.bfloat16, device=cuda_device)
+    q_out, k_out = buf[:t, :h], buf[:t, h:]
+    shifted = a["q"]._base[1:, :h], a["q"]._base[1:, h:h + hk]
+    for over in (dict(k_out=buf[:t, 1:1 + hk]), dict(k_out=buf[1:1 + t, :hk]), dict(q_out=a["q"]._base[:, hk:h + hk]),
+                 dict(k_out=a["q"][:, :hk]), dict(q_out=a["q"]._base[:, 1:1 + h]), dict(k_out=q_out[:, 2:])):
+        before = a["q"]._base.clone(), buf.clone()
+        with pytest.raises(ValueError, match="must not overlap"):
+            qk_norm_rope.launch(**{**a, "q_out": q_out, "k_out": k_out, **over})
+        assert torch.equal(a["q"]._base, before[0]) and torch.equal(buf, before[1])
+    short = {**a, "q": a["q"][:-1], "k": a["k"][:-1], "positions": a["positions"][:-1]}
+    for over in (dict(q_out=shifted[0]), dict(k_out=shifted[1])):
+        with pytest.raises(ValueError, match="must not overlap"):
+            qk_norm_rope.launch(**{**short, "q_out": q_out[:-1], "k_out": k_out[:-1], **over})
+    grads = [torch.randn(*a[n].shape, generator=g).bfloat16().to(cuda_device) for n in ("q", "k")]
+    dw = [torch.empty(d, device=cuda_device) for _ in range(2)]
+    into = dict(dq_out=grads[0], dk_out=grads[1], dq=q_out, dk=k_out, dq_weight=dw[0], dk_weight=dw[1])
+    for over in (dict(dk=grads[0][:, :hk]), dict(dq=a["q"]._base[:, hk:h + hk]), dict(dk=q_out[:, 1:1 + hk]),
+                 dict(dq_weight=buf.flatten()[2 * d:4 * d].view(torch.float32)),
+                 dict(dk_weight=buf.flatten()[h * d:(h + 2) * d].view(torch.float32))):
+        with pytest.raises(ValueError, match="must not overlap"):
+            qk_norm_rope.launch_backward(**{**a, **into, **over})
+    # Beside each other in one buffer they are taken.
+    qk_norm_rope.launch(**a, q_out=q_out, k_out=k_out)
+    assert torch.equal(q_out, want[0]) and torch.equal(k_out, want[1]) and not buf[t:].any()
+
+
+@pytest.mark.parametrize("d", [128, 37])
+def test_gradient_over_the_values(d, cuda_device):
+    a, g = make(300, 6, 2, d, 16, "bf16")
+    grads = [torch.randn(*a[n].shape, generator=g).bfloat16().to(cuda_device) for n in ("q", "k")]
+    want = backward(a, *grads)
+    got = backward(a, *grads, dq=a["q"], dk=a["k"])
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
+def test_two_heads_per_side_in_every_layout(cuda_device):
+    """q, k and v beside each other in every head, in place; heads in front of tokens."""
+    t, h, d = 50, 4, 64
+    a, _ = make(t, h, h, d, 32, "bf16", packed=False)
+    want = forward(a)
+    for shape, order in (((t, h, 3, d), (2, 0, 1, 3)), ((h, t, 3, d), (2, 1, 0, 3)), ((3, h, t, d), (0, 2, 1, 3))):
+        buf = torch.zeros(shape, dtype=torch.bfloat16, device=cuda_device)
+        q, k, v = buf.permute(order)
+        q.copy_(a["q"])
+        k.copy_(a["k"])
+        qk_norm_rope.launch(q, k, a["q_weight"], a["k_weight"], a["positions"], a["cos_sin"], q, k)
+        assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and not v.any()
