@@ -20,11 +20,27 @@ from flashattentionanycard_b200 import _native
 MAX_SLOTS, MAX_SIZE, RANKS = 1024, 1 << 30, (16, 32, 64, 128)
 
 
+def _moved_exponent(largest, scale):
+    """e of the power of two that an fp16 adapter's slot takes from its scale into b.
+
+    The kernels round scale (x @ A.T) to fp16, which holds 2^-24 to 65504.  With
+    the largest value of b 2^e in [1, 2) that product is past 65504 only where the
+    adapter's result is too, and what it loses below the smallest normal number
+    is a step of 2^-25 of the result.  Up, b 2^e is exact.  Down it may lose bits
+    of its smallest values, so b goes down only to bring a scale below one up to it."""
+    if not largest or not scale:
+        return 0
+    up = 1 - math.frexp(largest)[1]
+    return max(up, min(0, math.frexp(scale)[1] - 1))
+
+
 class AdapterBank:
     """Adapters of one [K, N] projection in ``slots`` device slots, ranks up to ``max_rank``.
 
     ``load`` copies an adapter in (on the current stream) and refuses values
-    that are not finite: rows of other adapters meet them as zero factors."""
+    that are not finite: rows of other adapters meet them as zero factors.  In
+    fp16 the slot's b and scale may differ from the loaded ones by a power of
+    two that their product does not see."""
 
     def __init__(self, slots, k, n, max_rank, dtype, device):
         import torch
@@ -71,6 +87,10 @@ class AdapterBank:
         largest = torch.linalg.vector_norm(a, float("inf")) + torch.linalg.vector_norm(b, float("inf")) * 0
         if not math.isfinite(largest.item()):
             raise ValueError("the adapter holds values that are not finite")
+        if self.dtype == torch.float16:
+            e = _moved_exponent(torch.linalg.vector_norm(b, float("inf")).item(), scale)
+            if e:
+                b, scale = b * 2.0**e, scale * 2.0**-e
         into_a, into_b = self.a[slot], self.b[slot]
         into_a[:r].copy_(a)
         into_b[:r].copy_(b)

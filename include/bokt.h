@@ -216,7 +216,8 @@ int bokt_rmsnorm_gemm(const void* X, const void* B_folded, void* C, float* row_s
  * own rank (rows past it are zero), 0 for an empty slot; ids int32 [M].  The
  * adapters in use are read once per row tile and join the projection's fp32
  * accumulator; scales[a] (x A_a^T) is rounded to the type (it is a tensor-core
- * operand), the sum once.  out must not overlap x.  lora_b must be finite:
+ * operand; in fp16 it must stay below 65,504 and lose little below 2^-14: move a
+ * power of two between scales[a] and B_a where it would not), the sum once.  out must not overlap x.  lora_b must be finite:
  * rows of other adapters multiply it by zero.  An id outside [-1, slots) or of an empty slot sets the
  * device status word (code 6) and its row gets x W alone.  rank: 16, 32, 64 or
  * 128; slots <= 1024; K and N multiples of 8; M, K and N up to 2^30; 16-byte

@@ -340,3 +340,51 @@ def test_offsets_past_32_bits(cuda_device):
     for block in out.view(t // 1000, 1000, -1):
         assert ((block[some].double() - ref).abs() <= tol).all()
     assert torch.isfinite(out[:1000]).all() and torch.isfinite(out[-1000:]).all()
+
+
+def parts(scale, b_size, x_size=1.0, t=40, k=264, n=136, rank=16, seed=3):
+    """One fp16 adapter on every row of a zero projection, so that the result is the adapter's alone."""
+    g = torch.Generator().manual_seed(seed)
+    x = (x_size * torch.randn(t, k, generator=g)).half().cuda()
+    a = (torch.randn(rank, k, generator=g) * k**-0.5 * x_size**0.5).half().cuda()
+    b = (b_size * torch.randn(rank, n, generator=g)).half().cuda()
+    bank = lora_gemm.AdapterBank(3, k, n, rank, torch.float16, "cuda")
+    bank.load(1, a, b, scale)
+    out = torch.full((t, n), float("nan"), dtype=torch.float16, device="cuda")
+    w, ids = torch.zeros(k, n, dtype=torch.float16, device="cuda"), torch.ones(t, dtype=torch.int32, device="cuda")
+    lora_gemm.launch(x, w, bank, ids, out)
+    return f64(x), f64(a), f64(b), f64(out), k
+
+
+@pytest.mark.parametrize("t", [40, 700])
+@pytest.mark.parametrize("scale, b_size, x_size", [
+    (1e6, 2e-6, 1.0), (-3e5, 1e-4, 1.0), (1.5, 1e-3, 3e3), (1.0, 6e-8, 3e3),  # x A^T, or its scaled form, past 65504
+    (2e-7, 3e3, 1.0), (1e-9, 6e4 / 6, 30.0), (3e-3, 200.0, 1e-3),              # below the smallest normal number
+    (1.0, 0.3, 1.0), (0.7, 1e3, 1e-2),
+])
+def test_fp16_scales_and_adapters_of_any_size(scale, b_size, x_size, t, cuda_device):
+    """What the scale and the second factor multiply to is in range, so the
+    result is, whatever each of them is.
+
+    With 2^e the power of two between the factors, h = scale 2^-e (x A^T) is off
+    by (K + 4) v of its absolute sum, half a step of |h| and half a subnormal
+    step, 2^-25; b = B 2^e by 2^-25 where e < 0 made it subnormal; the sum adds
+    (rank + 136) v of its size; the result is rounded once.  Whichever e is
+    taken, one that serves leaves |b| at most 2 where |scale| > 1, and |h| no
+    larger than x A^T where B is moved down."""
+    x, a, b, out, k = parts(scale, b_size, x_size, t)
+    sc = float(np.float32(scale))
+    up = max(0, -int(np.floor(np.log2(np.abs(b).max()))))
+    down = max(0, min(int(np.floor(np.log2(np.abs(b).max()))), -int(np.floor(np.log2(abs(sc))))))
+    e = up - down
+    h, bb = sc * 2.0**-e * (x @ a.T), np.abs(b) * 2.0**e
+    dh = (k + 4) * V * abs(sc) * 2.0**-e * (np.abs(x) @ np.abs(a).T)
+    dh = dh + 2.0**-11 * (np.abs(h) + dh) + 2.0**-25
+    db = 2.0**-25 if e < 0 else 0.0
+    size = (np.abs(h) + dh) @ (bb + db)
+    tol = dh @ (bb + db) + np.abs(h).sum(1, keepdims=True) * db + 152 * V * size
+    ref = sc * (x @ a.T) @ b
+    assert np.abs(ref).max() < 60000
+    assert np.all(np.abs(out - ref) <= tol + 2.0**-11 * (np.abs(ref) + tol) + 2.0**-25)
+    # The bound says something: it is a small part of the result's size.
+    assert np.median(tol) < 0.02 * np.sqrt((ref * ref).mean()) + 2.0**-25 * 16

@@ -122,3 +122,20 @@ def test_sizes_past_32_bits_are_refused():
     x, w, ids = torch.zeros(1, 16, dtype=BF), torch.zeros(16, 24, dtype=BF), torch.zeros(1, dtype=torch.int32)
     with pytest.raises(ValueError, match="rows"):
         lora_gemm.launch(x.expand(most + 1, 16), w, b, ids, torch.zeros(1, 24, dtype=BF).expand(most + 1, 24))
+
+
+@pytest.mark.parametrize("scale, size, e", [
+    (1.0, 1.5, 0), (0.5, 0.6, 1), (1e6, 2e-3, 9), (-4.0, 6e-8, 24), (1.0, 3e4, 0), (0.3, 3.0, -1), (1e-6, 3.0, -1),
+    (1e-6, 3e4, -14), (2.0**-3, 3e4, -3), (0.0, 3e4, 0), (1.0, 0.0, 0),
+])
+def test_fp16_slots_move_a_power_of_two_from_the_scale(scale, size, e):
+    """The product of scale and b is kept, the larger ones of b exactly."""
+    bk = bank(dtype=torch.float16)
+    a1, b1 = torch.randn(4, 16).half(), (torch.rand(4, 24) * size / 2).half()
+    b1[2, 5] = -size
+    bk.load(1, a1, b1, scale)
+    assert torch.equal(bk.b[1, :4].double(), (b1 * 2.0**e).half().double())
+    assert bk.scales[1] == torch.tensor(scale * 2.0**-e, dtype=torch.float32)
+    assert torch.equal(bk.a[1, :4], a1) and bk.ranks[1] == 4
+    if e >= 0:
+        assert torch.equal(bk.b[1, :4].double() * 2.0**-e, b1.double())
