@@ -78,6 +78,7 @@ class AdapterBank:
                 or a.shape != (r, self.k) or b.shape != (r, self.n):
             raise ValueError(f"shape mismatch: a {tuple(a.shape)}, b {tuple(b.shape)}; expected [r, {self.k}] "
                              f"and [r, {self.n}] with r in [1, {self.max_rank}]")
+        a, b = a.detach(), b.detach()  # trained parameters leave no graph on the bank
         if a.dtype != self.dtype or b.dtype != self.dtype:
             raise ValueError(f"the adapter must have the bank's dtype {self.dtype}")
         scale = float(scale)

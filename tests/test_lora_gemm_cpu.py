@@ -139,3 +139,24 @@ def test_fp16_slots_move_a_power_of_two_from_the_scale(scale, size, e):
     assert torch.equal(bk.a[1, :4], a1) and bk.ranks[1] == 4
     if e >= 0:
         assert torch.equal(bk.b[1, :4].double() * 2.0**-e, b1.double())
+
+
+def test_parameters_loaded_into_the_bank_leave_no_graph():
+    """A bank is storage: loading trained parameters records no history on it."""
+    b = bank()
+    a1 = torch.nn.Parameter(torch.randn(8, 16).to(BF))
+    b1 = torch.nn.Parameter(torch.randn(8, 24).to(BF))
+    b.load(0, a1, b1)
+    b.load(0, a1[:3], b1[:3])
+    for t in (b.a, b.b, b.scales, b.ranks):
+        assert not t.requires_grad and t.grad_fn is None
+    b.unload(0)
+    b.load(0, a1[:3], b1[:3])
+    assert torch.equal(b.a[0, :3], a1[:3]) and not b.a[0, 3:].any()
+
+
+def test_fp16_parameters_leave_no_graph_either():
+    b = bank(dtype=torch.float16)
+    a1, b1 = torch.nn.Parameter(torch.randn(8, 16).half()), torch.nn.Parameter(torch.full((8, 24), 0.25).half())
+    b.load(0, a1, b1, 1e5)
+    assert not (b.a.requires_grad or b.b.requires_grad or b.scales.requires_grad) and b.b[0, 0, 0] == 1
