@@ -263,3 +263,98 @@ def test_matches_the_routed_chain(cuda_device):
     combine(y, gates, out, router.inv_perm)
     mine = f64(run(a, topk))
     assert np.linalg.norm(f64(out) - mine) <= 2.0**-7 * np.linalg.norm(mine)
+
+
+def picked(a, topk):
+    """Experts of every token, fp64 order."""
+    return decoder.moe_gate(f64(a["logits"]), topk)[0]
+
+
+def cuts_tiles(t, k, inner, active):
+    """Whether the persistent kernel's first phase cuts its tiles: its rule on the device's SMs."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    tiles, steps = active * -(-inner // 128), -(-k // 64)
+    return t > 16 and -(-tiles // sms) * steps > tiles * steps // sms + 12
+
+
+# Few wide tiles, each shared by 16 and by 32 runs of k-steps (more than one
+# round of the partial sums' loads), and runs that end one tile and begin the
+# next; an expert of one or two rows beside ones of many.
+CUT = [(20, 4, 4096, 136, 2, 0.0), (17, 2, 8192, 72, 1, 3.0), (128, 160, 1032, 120, 8, 0.0), (33, 9, 2056, 264, 2, 4.0)]
+
+
+def make_cut(t, e, k, inner, topk, skew, dtype="bf16"):
+    a = make(t, e, k, inner, dtype, skew=skew)
+    ids = picked(a, topk)
+    assert cuts_tiles(t, k, inner, len(np.unique(ids)))
+    return a, np.bincount(ids.ravel(), minlength=e)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("shape", CUT)
+def test_layer_of_cut_tiles(shape, dtype, cuda_device):
+    t, e, k, inner, topk, skew = shape
+    a, rows = make_cut(*shape, dtype)
+    if skew:
+        assert rows.max() > 2 and ((rows > 0) & (rows <= 2)).any()
+    out = run(a, topk)
+    check(a, topk, out, dtype)
+    for _ in range(10):
+        assert torch.equal(out, run(a, topk))
+
+
+@pytest.mark.parametrize("shape", CUT)
+def test_cut_tiles_dirty_workspace_and_rows_that_are_not_finite(shape, cuda_device):
+    t, e, k, inner, topk, skew = shape
+    a, _ = make_cut(*shape)
+    want = run(a, topk)
+    need = moe_decode.workspace_bytes(t, e, k, inner, topk)
+    ids = picked(a, topk)
+    bad = {**a, "x": a["x"].clone()}
+    bad["x"][5, 3] = float("nan")
+    bad["x"][11, k - 1] = float("inf")
+    good = [i for i in range(t) if i not in (5, 11)]
+    for fill in (0, 255, 127):
+        ws = torch.full((need + 4096,), fill, dtype=torch.uint8, device=cuda_device)
+        out = torch.zeros(t + 16, k, dtype=torch.bfloat16, device=cuda_device)
+        moe_decode.launch(**a, out=out[8:8 + t], topk=topk, workspace=ws[:need])
+        assert torch.equal(out[8:8 + t], want)
+        assert not out[:8].any() and not out[8 + t:].any() and (ws[need:] == fill).all()
+        ws[:need] = fill
+        got = run(bad, topk, workspace=ws[:need])
+        assert torch.equal(got[good], want[good])
+        assert torch.isnan(got[5]).all() and not torch.isfinite(got[11]).any()
+    spoiled = int(ids[0, 0])
+    hit = torch.from_numpy((ids == spoiled).any(1))
+    a["w_gate_up"][spoiled, k - 1] = float("nan")
+    got = run(a, topk)
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], want[~hit])
+
+
+def test_cut_tiles_on_streams_and_in_graphs(cuda_device):
+    cases = [(make_cut(*s)[0], s[4]) for s in CUT]
+    want = [run(a, k) for a, k in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    outs = []
+    for turn in range(8):
+        for i, (a, k) in enumerate(cases):
+            with torch.cuda.stream(streams[(i + turn) % len(streams)]):
+                outs.append((i, run(a, k)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i, o in outs)
+    graphs = []
+    for a, k in cases:
+        out = torch.full_like(a["x"], float("nan"))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            moe_decode.launch(**a, out=out, topk=k)
+            moe_decode.launch(**a, out=out, topk=k)
+        graphs.append((graph, out))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for (_, o), w in zip(graphs, want))
