@@ -388,3 +388,72 @@ def test_two_heads_per_side_in_every_layout(cuda_device):
         k.copy_(a["k"])
         qk_norm_rope.launch(q, k, a["q_weight"], a["k_weight"], a["positions"], a["cos_sin"], q, k)
         assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and not v.any()
+
+
+def torch_forms(a, side, g, interleaved, eps=1e-6):
+    """fp64 on the GPU, apart from the kernels and from the oracle's indexing:
+    (forward, gradient of x, gradient of w, and the sums of absolute values that
+    the bounds are taken from), heads of one side."""
+    x, w, g = a[side].double(), a[side + "_weight"].double(), g.double()
+    d, rot = x.shape[2], a["cos_sin"].shape[1]
+    cs = a["cos_sin"].double()[a["positions"].long()][:, None]
+    turn = torch.complex(cs[..., : rot // 2], cs[..., rot // 2:])
+
+    def rotate(v, by, size=False):
+        z = v[..., :rot]
+        lo, hi = (z[..., 0::2], z[..., 1::2]) if interleaved else z.split(rot // 2, -1)
+        if size:
+            lo = hi = lo.abs() + hi.abs()
+        else:
+            z = torch.complex(lo, hi) * by
+            lo, hi = z.real, z.imag
+        z = torch.stack([lo, hi], -1).flatten(-2) if interleaved else torch.cat([lo, hi], -1)
+        rest = v[..., rot:]
+        return torch.cat([z, 2 * rest.abs() if size else rest], -1)
+
+    r = (x.square().mean(-1, keepdim=True) + eps).rsqrt()
+    n = x * r
+    back = rotate(g, turn.conj())
+    gw, ga = back * w, rotate(g, None, size=True)
+    dx = r * (gw - n * (gw * n).mean(-1, keepdim=True))
+    gaw = ga * w.abs()
+    size = r * (gaw + n.abs() * (gaw * n.abs()).mean(-1, keepdim=True))
+    return rotate(n * w, turn), rotate(n * w, None, size=True), dx, size, (back * n).sum((0, 1)), (ga * n.abs()).sum((0, 1))
+
+
+def close(got, ref, tol):
+    assert got.shape == ref.shape and bool(((got.double() - ref).abs() <= tol).all())
+
+
+# Enough head rows that a warp takes two or four batches of a token's heads
+# behind one load of the angles, on 8, 16 and 32 lanes a row; heads that do not
+# fill the batches.
+MANY = [(16500, 9, 3, 128, 96), (30100, 17, 3, 64, 32), (22000, 5, 2, 256, 64), (21900, 14, 2, 80, 80),
+        (61000, 9, 2, 48, 16)]
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("shape", MANY)
+def test_many_head_rows(shape, interleaved, cuda_device):
+    """Both directions over several batches a unit.
+
+    The weights' gradient: a lane adds its four rows of a batch and then the
+    batches of its units (two a unit; 296 blocks of 8 warps share the units); a
+    block adds the rows of at most 32 lane groups, and the last kernel at most
+    296 / 32 + 1 blocks and then 32 sums: depth 4 + batches + 32 + 10 + 32."""
+    t, h, hk, d, rot = shape
+    a, g = make(t, h, hk, d, rot, "bf16", seed=t)
+    grads = [torch.randn(*a[n].shape, generator=g).bfloat16().to(cuda_device) for n in ("q", "k")]
+    outs, got = forward(a, interleaved), backward(a, *grads, interleaved)
+    half = torch.finfo(torch.bfloat16).eps / 2 * (1 + 1e-3)
+    heads = 2 * 4 * 32 // (8 if d <= 64 else 16 if d <= 128 else 32)  # of a unit
+    depth = 78 + 2 * -(-t * (-(-h // heads) - (-hk // heads)) // (296 * 8))
+    for i, side in enumerate(("q", "k")):
+        y, near, dx, size, dw, dw_size = torch_forms(a, side, grads[i], interleaved)
+        close(outs[i], y, half * y.abs() + (d / 16 + 20) * U * near)
+        close(got[i], dx, half * dx.abs() + (d / 4 + 64) * U * size)
+        close(got[2 + i], dw, (depth + d / 16 + 20) * U * dw_size)
+        # A bound that a missing batch would not pass: one row's share of the sum.
+        assert float(((depth + d / 16 + 20) * U * dw_size).max()) < 0.05 * float(dw.abs().mean())
+    again = backward(a, *grads, interleaved)
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
