@@ -190,3 +190,41 @@ def test_operators_of_several_streams_at_once(cuda_device):
     torch.cuda.synchronize()
     for i, out in got:
         assert torch.equal(out, want[i]), i
+
+
+def test_training_pair_along_its_own_gradient(cuda_device):
+    """As above, along the fp64 gradient with noise, where a gradient of zero or
+    of the wrong sign is far off.
+
+    dq is rounded (2^-8 of every term).  Its g is rounded twice, as q_out and as
+    the difference: 2^-8 (|q_out| + |g|) of every element, which moves the slope
+    by its product with the forward form's change along the direction."""
+    t, h, d = 20, 3, 64
+    g = torch.Generator().manual_seed(0)
+    q = torch.randn(t, h, d, generator=g).to(BF).cuda()
+    k = q[:, :1].contiguous()
+    w = (1 + 0.2 * torch.randn(d, generator=g)).to(BF).cuda()
+    table = qk_norm_rope.rope_table(64, d, device="cuda")
+    pos = torch.arange(t, dtype=torch.int32, device="cuda")
+    target = torch.randn(t, h, d, generator=g).to(BF).cuda()
+    q_out, k_out, dq, dk = (torch.empty_like(x) for x in (q, k, q, k))
+    dw = [torch.empty(d, device="cuda") for _ in range(2)]
+    qk_norm_rope.launch(q, k, w, w, pos, table, q_out, k_out, 1e-3)
+    dout = (q_out.float() - target.float()).to(BF)
+    qk_norm_rope.launch_backward(dout, torch.zeros_like(k), q, k, w, w, pos, table, dq, dk, dw[0], dw[1], 1e-3)
+
+    def form(x, weight):
+        return decoder.qk_norm_rope(x, weight, np.arange(t), f64(table), 1e-3)
+
+    x, weight, goal, step = f64(q), f64(w), f64(target), 1e-6
+    rng = np.random.default_rng(0)
+    full = decoder.qk_norm_rope_backward(form(x, weight) - goal, x, weight, np.arange(t), f64(table), 1e-3)
+    round_g = 2.0**-8 * (np.abs(f64(q_out)) + np.abs(f64(dout)))
+    for mine, grad, move, rounding in ((f64(dq), full[0], lambda s, way: form(x + s * way, weight), 2.0**-8),
+                                       (f64(dw[0]), full[1], lambda s, way: form(x, weight + s * way), 1e-5)):
+        way = grad + 0.3 * np.sqrt((grad * grad).mean()) * rng.normal(size=grad.shape)
+        up, down = move(step, way), move(-step, way)
+        slope = 0.5 * (((up - goal) ** 2).sum() - ((down - goal) ** 2).sum()) / (2 * step)
+        tol = rounding * np.abs(mine * way).sum() + (round_g * np.abs(up - down)).sum() / (2 * step) + 1e-4
+        assert abs((mine * way).sum() - slope) <= tol
+        assert abs(slope) > 4 * tol  # zero, or the other sign, would not pass
