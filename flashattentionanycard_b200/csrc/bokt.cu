@@ -2016,7 +2016,11 @@ constexpr int kLoraFewRows = 256;
 constexpr int kLoraStreamRows = 1024;
 // Sizes whose tile arithmetic stays in 32 bits.
 constexpr int kLoraMaxSize = 1 << 30;
-// Shared memory left to a shrink CTA (rank 16: 9 KB of partials, 7 KB of lists).
+// Shared memory left beside the W stream: a shrink CTA of rank 16 (9 KB of
+// partials, 7 KB of lists, 1 KB of the system's).  Rank 32 takes 26 KB and rank 64
+// or more 44 KB, which only what the stream's whole stages leave over may hold:
+// beside tiles of 32 rows neither, of 64 and 128 rows rank 32, of the others both.
+// Where they do not fit, the stream's CTA starts when the shrink's leaves its SM.
 constexpr int kLoraShrinkSmem = 20 * 1024;
 
 struct LoraPlan {

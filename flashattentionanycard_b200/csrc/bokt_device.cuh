@@ -41,9 +41,15 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
 // Programmatic dependent launch.  Every kernel of the library is launched with
 // programmatic stream serialization, so it may start while the previous
 // kernel in the stream drains.  pdl_wait() blocks until that kernel has
-// completed and its memory is visible: every kernel calls it before its first
-// global-memory access.  pdl_allow_next() lets the next kernel begin its own
-// launch early.  Both are no-ops when the kernel was launched without PDL.
+// completed and its memory is visible: a kernel calls it before its first
+// global-memory access.  One exception: the second kernel of an operator of two
+// may read what the operator was given before its wait, if the first lets it go
+// (pdl_allow_next) only after a wait of its own, since all that came before the
+// pair is complete then (lora_stream_kernel and lora_tc2_kernel read x and W,
+// moe_few_down_kernel logits and weights).  It waits before it reads what the
+// first kernel writes and before it writes anything.  pdl_allow_next() lets the
+// next kernel begin its own launch early.  Both are no-ops when the kernel was
+// launched without PDL.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ void pdl_allow_next() {

@@ -22,9 +22,14 @@
 //       one; a cluster of C CTAs splits K and reduces through distributed shared
 //       memory.
 //   lora_tc2_kernel     many tokens: the CTA-pair GEMM's 256 x 256 tiles.
-// Both products start on x and W while the shrink kernel still runs: it lets
-// its dependents go only after its own wait, so everything before it is
-// complete by then; they wait for it before the first H.
+// Both products start on x and W while the shrink kernel still runs (the stream
+// on the SMs that hold a CTA of each, see kLoraShrinkSmem): it lets its
+// dependents go only after its own wait, so everything before it is complete by
+// then; they wait for it before the first H.
+// Held in 16 bits: H.  Its scale is applied in fp32 before that rounding; in fp16
+// the bank keeps both in range.  Scratch: H for min(slots, tile rows) adapters a
+// row tile, whichever of them the batch uses.
+// lora_shrink_kernel spills 8 bytes at rank 64 (128 registers for two CTAs an SM).
 #pragma once
 
 #include "bokt_device.cuh"

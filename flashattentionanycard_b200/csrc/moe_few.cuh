@@ -17,9 +17,10 @@
 // Both sums run in rank order.  Measured against the persistent kernel (us a
 // call): 8 experts x [1024, 2 x 2048], top 2: one token 13.2 and 22.7, four 25
 // and 33, sixteen 33 and 35; 128 x [2048, 2 x 768], top 8: one token 24 and 40,
-// four 58 and 67; 16 x [4096, 2 x 14336], top 2: one token 122 and 123.  Past 16
-// tokens routing in every CTA costs more than it saves (37 tokens of 12 experts:
-// 45 and 35).
+// four 58 and 67; 16 x [4096, 2 x 14336], top 2: one token 122 and 123.  16 tokens
+// are what one box of x and 16 accumulator columns an expert hold; a form for
+// more was slower where it was measured (37 tokens of 12 experts: 45 and 35, every
+// CTA routes all tokens).
 #pragma once
 
 #include "moe_decode.cuh"

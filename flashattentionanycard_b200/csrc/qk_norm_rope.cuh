@@ -18,10 +18,17 @@
 // shuffles, and a rotation partner is another lane's register.  A warp takes
 // 32 / L x R x loops heads of one token: the token's angles are loaded once
 // into 16 registers and serve all of them, and R row loads are in flight per
-// lane.  Measured at (32 + 8) heads x 128 bf16: forward of 16384 tokens 62-63 us,
-// 5.4 TB/s with the table (without overlap of launches: one loop of R = 4 77 us,
-// two 68, four 64; R = 2 70-82); backward of 8192 tokens 58 us, 4.4 TB/s (one
-// loop 64, two 57, four 58; R = 2 58-83; 24 warps an SM instead of 16: 62).
+// lane.  Measured at (32 + 8) heads x 128 bf16: forward of 16384 tokens 62-63 us
+// back to back in a graph, 5.4 TB/s with the table, 67-70 in single calls (without
+// overlap of launches: one loop of R = 4 77 us, two 68, four 64; R = 2 70-82);
+// backward of 8192 tokens 58 us, 4.4 TB/s (one loop 64, two 57, four 58; R = 2
+// 58-83; 24 warps an SM instead of 16: 62).  The forward kernel of R = 4 spills 4-32
+// bytes under its 64 registers (32 warps an SM), but for neighbours that all turn;
+// the backward kernel none.
+// The strided kernel below (other head sizes, rotations and alignments) is not
+// tuned: one warp a row, 2-byte loads, at most 8 warps an SM.  Forward and backward
+// in us: 4096 tokens of (32 + 8) x 512 924 and 1057 (0.37 and 0.48 TB/s), 16384 of
+// 96 with rot 24 924 and 1124, 16384 of 128 off 16 bytes 1184 and 1335.
 #pragma once
 
 #include "bokt_device.cuh"

@@ -110,7 +110,10 @@ class AdapterBank:
 
 
 def workspace_bytes(m, bank):
-    """Device scratch of one call with m rows on the current device."""
+    """Device scratch of one call with m rows on the current device: sized for a
+    batch that uses as many of the bank's slots as it can, about
+    2 m rank min(slots, 256) bytes for many rows (8192 rows and 256 slots of rank
+    128: 0.5 GB)."""
     lib = _native.load()
     n = int(lib.bokt_lora_gemm_workspace_bytes(int(m), bank.n, bank.k, bank.slots, bank.rank))
     if n < 0:

@@ -224,7 +224,9 @@ int bokt_rmsnorm_gemm(const void* X, const void* B_folded, void* C, float* row_s
  * aligned pointers.
  * workspace: bokt_lora_gemm_workspace_bytes(...) bytes of device scratch,
  * 256-byte aligned, contents free before and after; calls that overlap on the
- * GPU need one each.  The product is that of kernels/gemm.py:7-40; adapters
+ * GPU need one each.  It is sized for the worst batch of the bank: about
+ * 2 * M * rank * min(slots, 256) bytes for many rows (up to 128 adapters a row
+ * tile for few), 0.5 GB for 8192 rows with 256 slots of rank 128.  The product is that of kernels/gemm.py:7-40; adapters
  * have no counterpart in the reference.
  */
 int64_t bokt_lora_gemm_workspace_bytes(int M, int N, int K, int slots, int rank);
@@ -527,7 +529,7 @@ int bokt_moe_combine(const void* y, int64_t y_rows, const int32_t* rows, const f
  *   out[t] = sum_j gate_j (silu(x[t] Wg_j) * (x[t] Wu_j)) Wd_j
  * with [Wg | Wu] = w_gate_up[e] ([K, 2 I]) and Wd = w_down[e] ([I, K]).  The
  * weights of every expert in use are read once.  silu(gate) * up is rounded to
- * dtype (it is a tensor-core operand); the experts' results are summed in fp32
+ * dtype (it is a tensor-core operand; in fp16 it is infinite past 65,504); the experts' results are summed in fp32
  * and rounded once.  x, out [tokens, K] (out may be x); logits [tokens, E] fp16/bf16/fp32.
  * A NaN logit makes its token's gates and output NaN.  tokens <= 128,
  * topk <= 8, E <= 1024, K and I multiples of 8, 16-byte aligned pointers (else
