@@ -1661,7 +1661,9 @@ int qk_norm_rope_impl(bokt::QkArgs* a, const int64_t* strides, int interleaved, 
              aligned16(a->cos_sin);
   int rc;
   if (!empty) {
-    if (!strides || !a->positions || !a->cos_sin) return fail(BOKT_ERR_INVALID, "null pointer");
+    // A table without rows has no memory: every position is outside it.
+    if (!strides || !a->positions || (!a->cos_sin && a->table_rows > 0))
+      return fail(BOKT_ERR_INVALID, "null pointer");
     for (int i = 0; i < 2; ++i) {
       bokt::QkSide& s = a->side[i];
       if (s.heads && (!s.x || !s.w || !s.out || (grad && !s.g)))

@@ -457,3 +457,16 @@ def test_many_head_rows(shape, interleaved, cuda_device):
         assert float(((depth + d / 16 + 20) * U * dw_size).max()) < 0.05 * float(dw.abs().mean())
     again = backward(a, *grads, interleaved)
     assert all(torch.equal(x, y) for x, y in zip(got, again))
+
+
+@pytest.mark.parametrize("d", [64, 37])
+def test_every_position_is_outside_an_empty_table(d, cuda_device):
+    a, g = make(5, 3, 2, d, 16, "bf16")
+    a["cos_sin"] = qk_norm_rope.rope_table(0, 16, device=cuda_device)
+    q_out, k_out = forward(a)
+    assert _native.device_status(reset=True)[0] == 5
+    assert torch.isnan(q_out).all() and torch.isnan(k_out).all()
+    grads = [torch.randn(*a[n].shape, generator=g).bfloat16().to(cuda_device) for n in ("q", "k")]
+    dq, dk, *dw = backward(a, *grads)
+    assert _native.device_status(reset=True)[0] == 5
+    assert torch.isnan(dq).all() and torch.isnan(dk).all() and not dw[0].any() and not dw[1].any()
