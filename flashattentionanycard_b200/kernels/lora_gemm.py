@@ -73,7 +73,7 @@ class AdapterBank:
         import torch
 
         slot = self._slot(slot)
-        r = a.shape[0]
+        r = a.shape[0] if a.dim() else 0
         if a.dim() != 2 or b.dim() != 2 or not 1 <= r <= self.max_rank \
                 or a.shape != (r, self.k) or b.shape != (r, self.n):
             raise ValueError(f"shape mismatch: a {tuple(a.shape)}, b {tuple(b.shape)}; expected [r, {self.k}] "
@@ -131,6 +131,8 @@ def launch(x, w, bank, ids, out, workspace=None):
     torch's allocator."""
     import torch
 
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError(f"x and w must have two dimensions, got {tuple(x.shape)} and {tuple(w.shape)}")
     m, k = x.shape
     n = w.shape[1]
     if w.shape[0] != k or out.shape != (m, n):

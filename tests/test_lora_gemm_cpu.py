@@ -160,3 +160,12 @@ def test_fp16_parameters_leave_no_graph_either():
     a1, b1 = torch.nn.Parameter(torch.randn(8, 16).half()), torch.nn.Parameter(torch.full((8, 24), 0.25).half())
     b.load(0, a1, b1, 1e5)
     assert not (b.a.requires_grad or b.b.requires_grad or b.scales.requires_grad) and b.b[0, 0, 0] == 1
+
+
+def test_other_numbers_of_dimensions_are_refused():
+    for shape in ((), (16,), (1, 16, 1)):
+        with pytest.raises(ValueError, match="shape mismatch"):
+            bank().load(0, torch.zeros(shape, dtype=BF), torch.zeros(1, 24, dtype=BF))
+    for over in (dict(w=torch.zeros(16, dtype=BF)), dict(x=torch.zeros(16, dtype=BF)), dict(x=torch.zeros(3, 1, 16, dtype=BF))):
+        with pytest.raises(ValueError, match="dimensions"):
+            call(**over)
