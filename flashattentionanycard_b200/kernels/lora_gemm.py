@@ -24,10 +24,11 @@ def _moved_exponent(largest, scale):
     """e of the power of two that an fp16 adapter's slot takes from its scale into b.
 
     The kernels round scale (x @ A.T) to fp16, which holds 2^-24 to 65504.  With
-    the largest value of b 2^e in [1, 2) that product is past 65504 only where the
-    adapter's result is too, and what it loses below the smallest normal number
-    is a step of 2^-25 of the result.  Up, b 2^e is exact.  Down it may lose bits
-    of its smallest values, so b goes down only to bring a scale below one up to it."""
+    the largest value of b 2^e in [1, 2), and its rows of like size, that product
+    is past 65504 only where the adapter's result is too, and what it loses below
+    the smallest normal number is a step of 2^-25 of the result.  Up, b 2^e is
+    exact.  Down it may lose bits of its smallest values, so b goes down only to
+    bring a scale below one up to it."""
     if not largest or not scale:
         return 0
     up = 1 - math.frexp(largest)[1]

@@ -12,9 +12,9 @@ the rate at which the weights of the experts in use arrive from HBM:
 with ``w_gate_up`` [E, K, 2 I] holding the gate columns and then the up columns
 of every expert, ``w_down`` [E, I, K], and g_j = p[e_j], divided by their sum
 with ``renormalize``.  silu(..) * (..) is rounded to the element type between the
-products (in fp16 within 65,504), the result once more.  The reference has the grouped product alone
-(``bo_kernel_tuner/kernels/moe_grouped_gemm.py:61-65``) and leaves the rest of
-the layer outside.
+products (in fp16 within 65,504), the result once more.  The reference has the
+grouped product alone (``bo_kernel_tuner/kernels/moe_grouped_gemm.py:61-65``)
+and leaves the rest of the layer outside.
 """
 
 from flashattentionanycard_b200 import _native

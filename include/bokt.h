@@ -217,8 +217,9 @@ int bokt_rmsnorm_gemm(const void* X, const void* B_folded, void* C, float* row_s
  * adapters in use are read once per row tile and join the projection's fp32
  * accumulator; scales[a] (x A_a^T) is rounded to the type (it is a tensor-core
  * operand; in fp16 it must stay below 65,504 and lose little below 2^-14: move a
- * power of two between scales[a] and B_a where it would not), the sum once.  out must not overlap x.  lora_b must be finite:
- * rows of other adapters multiply it by zero.  An id outside [-1, slots) or of an empty slot sets the
+ * power of two between scales[a] and B_a where it would not), the sum once.  out
+ * must not overlap x.  lora_b must be finite: rows of other adapters multiply it
+ * by zero.  An id outside [-1, slots) or of an empty slot sets the
  * device status word (code 6) and its row gets x W alone.  rank: 16, 32, 64 or
  * 128; slots <= 1024; K and N multiples of 8; M, K and N up to 2^30; 16-byte
  * aligned pointers.
@@ -226,8 +227,8 @@ int bokt_rmsnorm_gemm(const void* X, const void* B_folded, void* C, float* row_s
  * 256-byte aligned, contents free before and after; calls that overlap on the
  * GPU need one each.  It is sized for the worst batch of the bank: about
  * 2 * M * rank * min(slots, 256) bytes for many rows (up to 128 adapters a row
- * tile for few), 0.5 GB for 8192 rows with 256 slots of rank 128.  The product is that of kernels/gemm.py:7-40; adapters
- * have no counterpart in the reference.
+ * tile for few), 0.5 GB for 8192 rows with 256 slots of rank 128.  The product is
+ * that of kernels/gemm.py:7-40; adapters have no counterpart in the reference.
  */
 int64_t bokt_lora_gemm_workspace_bytes(int M, int N, int K, int slots, int rank);
 int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void* lora_b,
@@ -246,8 +247,8 @@ int bokt_lora_gemm(const void* x, const void* W, const void* lora_a, const void*
  * whose cosine is cos_sin[p][i] and whose sine is cos_sin[p][rot / 2 + i]
  * (fp32 [table_rows, rot]).  fp32 arithmetic, one rounding.  q_out / k_out may
  * be q / k themselves (same strides); any other overlap of an output with
- * another or with q or k is BOKT_ERR_OVERLAP.  A position outside the table sets the
- * device status word (code 5) and leaves that token's heads unwritten.
+ * another or with q or k is BOKT_ERR_OVERLAP.  A position outside the table sets
+ * the device status word (code 5) and leaves that token's heads unwritten.
  * strides[8]: q row, q head, q_out row, q_out head, then the same of k.
  * tokens * (heads + kv_heads) up to 2^31 - 2^16; dim in [2, 1024], rot even;
  * dim a multiple of 8 up to 256 with 16-byte aligned rows and rot a multiple
@@ -264,8 +265,8 @@ int bokt_qk_norm_rope(const void* q, const void* k, const void* q_weight, const 
 /*
  * Gradients of bokt_qk_norm_rope: dq, dk (may be dq_out / dk_out, or q / k,
  * themselves; any other overlap is BOKT_ERR_OVERLAP) and the weights' gradients
- * dq_weight, dk_weight (fp32 [dim], apart from each other and from dq and dk, overwritten;
- * summed in a fixed order for a given device and shape).  The row statistics
+ * dq_weight, dk_weight (fp32 [dim], apart from each other and from dq and dk,
+ * overwritten; summed in a fixed order for a given device and shape).  The row statistics
  * are recomputed from q and k.  strides[12]: q row, q head, dq row, dq head,
  * dq_out row, dq_out head, then the same of k.  A token whose position is
  * outside the table contributes nothing and its dq / dk rows are left
@@ -529,8 +530,8 @@ int bokt_moe_combine(const void* y, int64_t y_rows, const int32_t* rows, const f
  *   out[t] = sum_j gate_j (silu(x[t] Wg_j) * (x[t] Wu_j)) Wd_j
  * with [Wg | Wu] = w_gate_up[e] ([K, 2 I]) and Wd = w_down[e] ([I, K]).  The
  * weights of every expert in use are read once.  silu(gate) * up is rounded to
- * dtype (it is a tensor-core operand; in fp16 it is infinite past 65,504); the experts' results are summed in fp32
- * and rounded once.  x, out [tokens, K] (out may be x); logits [tokens, E] fp16/bf16/fp32.
+ * dtype (it is a tensor-core operand; in fp16 it is infinite past 65,504); the
+ * experts' results are summed in fp32 and rounded once.  x, out [tokens, K] (out may be x); logits [tokens, E] fp16/bf16/fp32.
  * A NaN logit makes its token's gates and output NaN.  tokens <= 128,
  * topk <= 8, E <= 1024, K and I multiples of 8, 16-byte aligned pointers (else
  * BOKT_ERR_UNSUPPORTED: larger batches go through bokt_moe_topk_gate,
